@@ -395,6 +395,110 @@ int ypk_transpose_16bit(const void *src, void *dst, int32_t rows, int32_t cols, 
 int ypk_argmax_noalloc(const void *logits_bf16, int32_t batch, int32_t vocab, int64_t ld,
                        int64_t *out_tokens, void *stream);
 
+/* ---- Operators of a serving step that need no handle and no graph --------------------------
+ * For hosts that run their own loop around (or instead of) the persistent kernel, over the
+ * same paged K/V cache and the same request tables.  Every call is enqueued on `stream` and
+ * does not wait; all pointers are device pointers on the current device, the stream's own; the
+ * calls allocate nothing, keep nothing from one call for the next and may be captured into a
+ * graph.  Arguments that the host can check are refused with YPK_ERR_INVALID or
+ * YPK_ERR_UNSUPPORTED before anything is enqueued.  What stands in device memory (page numbers,
+ * lengths) is checked by the kernels: a broken entry never becomes an address, its token is
+ * left out, and a bit of *status tells. */
+
+/* Bits that the kernels set in ypk_paged_cache.status. */
+#define YPK_PAGED_BAD_TABLE 1    /* page offsets that run backwards or past the page list, or a
+                                    last_page_len outside 0..page_size: the request counts as
+                                    empty                                                     */
+#define YPK_PAGED_BAD_PAGE 2     /* a page number outside the pool: its tokens are left out     */
+#define YPK_PAGED_BAD_POSITION 4 /* a position outside the rotary tables: the token is dropped  */
+#define YPK_PAGED_BAD_LENGTH 8   /* more new tokens than the request is long: they are dropped  */
+
+/* One layer's paged K/V cache and the tables of the requests in it, as the persistent kernel
+ * keeps them.  Request r owns the pages indices[indptr[r] .. indptr[r + 1]) in order and is
+ * (pages - 1) * page_size + last_page_len[r] tokens long, new tokens included; no pages: an
+ * empty slot.  k and v are [num_pages][page_size][num_kv_heads][head_dim] by the given strides
+ * (in elements, the same for both, each a multiple of 8, head_dim contiguous), 16-byte
+ * aligned.  Any page_size from 1; head_dim 64, 128 or 256; at most 4096 requests. */
+typedef struct ypk_paged_cache {
+  void *k, *v;
+  int64_t stride_page, stride_token, stride_head;
+  const int32_t *indptr;        /* [num_requests + 1]                              */
+  const int32_t *indices;       /* [num_indices]                                   */
+  const int32_t *last_page_len; /* [num_requests]                                  */
+  const int32_t *qo_indptr;     /* [num_requests + 1]: rows of the new tokens of each request;
+                                   needed by ypk_paged_append only                 */
+  int32_t *status;              /* error bits are or-ed into it; may be NULL       */
+  int32_t dtype;                /* YPK_BF16 or YPK_F16                             */
+  int32_t num_pages, page_size, num_kv_heads, head_dim;
+  int32_t num_requests, num_indices;
+} ypk_paged_cache;
+
+/* Operands of ypk_paged_append.  Strides in elements, each a multiple of 8; pointers 16-byte
+ * aligned; the head dimension is contiguous everywhere.  Query head h is head h % group of group
+ * h / group, group = num_q_heads / num_kv_heads, so that the rows of a fused projection
+ * ([q heads of the group | k | v] per K/V head) are taken as they lie. */
+typedef struct ypk_paged_append_args {
+  const void *k, *v;            /* [num_tokens][num_kv_heads][head_dim]            */
+  const void *q;                /* [num_tokens][group..][head_dim], or NULL        */
+  void *q_out;                  /* rotated queries [num_tokens][num_q_heads][head_dim]; may be q */
+  const void *cos, *sin;        /* [max_positions][rot_dim]; NULL: no rotation     */
+  const void *q_norm, *k_norm;  /* [head_dim] in the cache's type; NULL: no norm   */
+  int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+  int64_t q_stride_token, q_stride_group, q_stride_head;
+  int64_t q_out_stride_token, q_out_stride_group, q_out_stride_head;
+  int64_t table_stride;         /* elements from one position's row to the next    */
+  int32_t num_tokens, num_q_heads;
+  int32_t rot_dim;              /* first rot_dim dimensions of a head are rotated; multiple of 16 */
+  int32_t max_positions;
+  int32_t table_dtype;          /* the cache's dtype or YPK_F32                    */
+  float eps;                    /* of the norms                                    */
+} ypk_paged_append_args;
+
+/* Writes the new tokens' K and V rows into the cache (the reference does this inside its
+ * attention task only, tasks/blackwell/attention_sm100.cuh:349-420): row j of request r's rows
+ * [qo_indptr[r], qo_indptr[r + 1]) goes to position length - rows + j.  On the way K, and Q if
+ * given, are RMS-normalised over the head dimension (where a weight is given) and rotated by
+ * halves: y[i] = x[i] cos[i] - x[i + h] sin[i], y[i + h] = x[i + h] cos[i + h] + x[i] sin[i + h],
+ * h = rot_dim / 2, in 32 bits with one rounding at the end.  Rows of k, v and q behind
+ * qo_indptr[num_requests] are not read into anything; the rows of q_out there stay as they
+ * were, and so do those of dropped tokens. */
+int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_append_args *args, void *stream);
+
+/* Operands of ypk_paged_decode. */
+typedef struct ypk_paged_decode_args {
+  const void *q;                /* [rows][group..][head_dim], grouped as in ypk_paged_append */
+  void *out;                    /* [rows][num_q_heads][head_dim]                   */
+  float *lse;                   /* [rows][num_q_heads] contiguous, or NULL         */
+  void *workspace;              /* ypk_paged_decode_workspace bytes, 16-byte aligned; holds
+                                   nothing between calls, not shared by calls that overlap */
+  uint64_t workspace_bytes;
+  int64_t q_stride_token, q_stride_group, q_stride_head;
+  int64_t out_stride_token, out_stride_group, out_stride_head;
+  int32_t rows, num_q_heads;
+  int32_t window;               /* > 0: only the last `window` positions are seen  */
+  float scale;                  /* of q.k                                          */
+} ypk_paged_decode_args;
+
+/* Attention of one new token per request over the cached positions (its own included): row r of
+ * q belongs to request r, r < rows <= num_requests; rows of out behind them stay as they were.
+ * out = sum_p softmax_p(scale q.k_p) v_p, lse = ln sum_p exp(scale q.k_p).  A request without
+ * positions gives zeros and -infinity. */
+int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_decode_args *args, void *stream);
+/* Workspace of such a call on the current device for any number of rows and any lengths. */
+int ypk_paged_decode_workspace(const ypk_paged_cache *cache, int32_t num_q_heads, uint64_t *bytes);
+
+/* Log probabilities of given tokens under softmax(logits[r, 0:vocab]):
+ * logprob[r] = log p(tokens[r]) (-infinity for a token outside [0, vocab)), entropy[r] =
+ * -sum p log p in nats, and the top_k (0..32) most probable tokens in falling order, the lower
+ * column first on ties: top_logprob, top_token [rows][top_k].  logits: dtype YPK_BF16, YPK_F16
+ * or YPK_F32, row stride ld elements, aligned to its element; columns from vocab to ld (the
+ * padding of an lm_head) are not looked at.  Columns of -infinity are ruled out; in a row that
+ * has no others every log probability is -infinity and the entropy 0.  A row with a NaN or
+ * +infinity gives NaN (its top tokens: NaN counts as lowest). */
+int ypk_token_logprobs(const void *logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t ld,
+                       const int64_t *tokens, int32_t top_k, float *logprob, float *entropy,
+                       float *top_logprob, int64_t *top_token, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,260 @@
+"""The serving operators without a GPU: what their host side refuses, through Python and through
+the C ABI, and the index arithmetic of the paged cache on good and broken tables."""
+import ctypes as C
+import os
+import shutil
+import subprocess
+
+import pytest
+import torch
+
+import yirage_b200 as yr
+from yirage_b200 import _native as N
+from yirage_b200 import llama
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def meta(requests=2, pages=4):
+    i32 = dict(dtype=torch.int32)
+    return {"qo_indptr_buffer": torch.tensor([0, 1, 2][:requests + 1], **i32),
+            "paged_kv_indptr_buffer": torch.tensor([0, 2, 4][:requests + 1], **i32),
+            "paged_kv_indices_buffer": torch.arange(pages, **i32),
+            "paged_kv_last_page_len_buffer": torch.tensor([3, 5][:requests], **i32)}
+
+
+def cache(dtype=torch.bfloat16, heads=2, dim=128, **kw):
+    k = torch.zeros(4, 16, heads, dim, dtype=dtype)
+    return yr.PagedKVCache(k, k.clone(), kw.get("meta", meta()))
+
+
+def test_cache_refuses_what_it_cannot_address(native_lib):
+    k = torch.zeros(4, 16, 2, 128, dtype=torch.bfloat16)
+    good = meta()
+    with pytest.raises(ValueError, match="must both be"):
+        yr.PagedKVCache(k, torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16), good)
+    with pytest.raises(TypeError, match="bfloat16 or float16"):
+        yr.PagedKVCache(k.float(), k.float(), good)
+    with pytest.raises(TypeError, match="bfloat16 or float16"):
+        yr.PagedKVCache(k, k.half(), good)
+    with pytest.raises(ValueError, match="same strides"):
+        yr.PagedKVCache(k, k.transpose(1, 2).contiguous().transpose(1, 2), good)
+    with pytest.raises(ValueError, match="same strides"):
+        t = torch.zeros(4, 16, 128, 128, dtype=torch.bfloat16).transpose(2, 3)
+        yr.PagedKVCache(t, t, good)
+    for key in ("paged_kv_indptr_buffer", "paged_kv_indices_buffer", "paged_kv_last_page_len_buffer"):
+        with pytest.raises(ValueError, match=f"'{key}' is missing"):
+            yr.PagedKVCache(k, k, {a: b for a, b in good.items() if a != key})
+        with pytest.raises(TypeError, match="int32"):
+            yr.PagedKVCache(k, k, dict(good, **{key: good[key].long()}))
+    with pytest.raises(ValueError, match="3 wanted"):
+        yr.PagedKVCache(k, k, dict(good, paged_kv_indptr_buffer=torch.zeros(4, dtype=torch.int32)))
+    with pytest.raises(TypeError, match="int32 vector"):
+        yr.PagedKVCache(k, k, dict(good, paged_kv_indices_buffer=torch.zeros(8, dtype=torch.int32)[::2]))
+
+
+def test_append_refusals(native_lib):
+    c = cache()
+    r = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype)
+    k, q = r(2, 2, 128), r(2, 8, 128)
+    table = r(64, 128)
+    for err, what, args in (
+            (TypeError, "k is torch.float16", dict(k=k.half())),
+            (ValueError, "k must be", dict(k=r(2, 3, 128))),
+            (ValueError, "k must be", dict(k=r(2, 2, 64))),
+            (ValueError, "v has|v 3", dict(v=r(3, 2, 128))),
+            (ValueError, "q has 3 rows", dict(q=r(3, 8, 128))),
+            (ValueError, "q must be", dict(q=r(2, 7, 128))),
+            (ValueError, "q must be", dict(q=r(2, 4, 2, 128))),
+            (ValueError, "rows and heads", dict(q=q, q_out=r(2, 4, 128))),
+            (ValueError, "must not overlap", dict(q=q, q_out=r(2, 1, 128).expand(2, 8, 128))),
+            (ValueError, "come with q", dict(q_out=q)),
+            (ValueError, "come with q", dict(q_norm=r(128))),
+            (ValueError, "come together", dict(cos=table)),
+            (TypeError, "cos and sin must both", dict(cos=table.half(), sin=table.half())),
+            (ValueError, "alike", dict(cos=table, sin=r(32, 128))),
+            (ValueError, "k_norm must be", dict(k_norm=r(64))),
+            (RuntimeError, "no CPU execution path", dict(q=q, cos=table, sin=table))):
+        call = dict(dict(k=k, v=k), **args)
+        with pytest.raises(err, match=what):
+            c.append(call.pop("k"), call.pop("v"), **call)
+    no_rows = cache(meta={a: b for a, b in meta().items() if a != "qo_indptr_buffer"})
+    with pytest.raises(ValueError, match="qo_indptr_buffer"):
+        no_rows.append(k, k)
+
+
+def test_decode_and_logprob_refusals(native_lib):
+    c = cache()
+    r = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype)
+    q = r(2, 8, 128)
+    for err, what, args, kw in (
+            (ValueError, "3 rows, the tables 2", (r(3, 8, 128),), {}),
+            (TypeError, "q is torch.float16", (q.half(),), {}),
+            (ValueError, "shape of q", (q,), dict(out=r(2, 4, 128))),
+            (ValueError, "must not overlap", (q,), dict(out=r(1, 8, 128).expand(2, 8, 128)))):
+        with pytest.raises(err, match=what):
+            c.decode(*args, **kw)
+    x, t = r(4, 100), torch.zeros(4, dtype=torch.int64)
+    for err, what, args, kw in (
+            (TypeError, "logits are torch.int64", (x.long(), t), {}),
+            (ValueError, "contiguous rows", (r(100, 4).t(), t), {}),
+            (ValueError, "contiguous rows", (r(400), t), {}),
+            (ValueError, "valid_cols 101 of 100", (x, t), dict(valid_cols=101)),
+            (ValueError, "valid_cols 0 of 100", (x, t), dict(valid_cols=0)),
+            (ValueError, "must not overlap", (r(1, 100).expand(4, 100), t), {}),
+            (TypeError, "tokens must be int64", (x, t.int()), {}),
+            (ValueError, r"tokens must be a contiguous \[4\]", (x, torch.zeros(5, dtype=torch.int64)), {}),
+            (RuntimeError, "no CPU execution path", (x, t), dict(top_k=3))):
+        with pytest.raises(err, match=what):
+            yr.token_logprobs(*args, **kw)
+
+
+def c_cache(**kw):
+    base = dict(k=0x10000, v=0x20000, stride_page=16 * 256, stride_token=256, stride_head=128, indptr=0x30000,
+                indices=0x30000, last_page_len=0x30000, qo_indptr=0x30000, status=None, dtype=N.BF16, num_pages=4,
+                page_size=16, num_kv_heads=2, head_dim=128, num_requests=2, num_indices=4)
+    return N.PagedCache(**dict(base, **kw))
+
+
+def test_c_abi_refuses_before_it_enqueues(native_lib):
+    """The pointers below point nowhere: a call that got past its checks would show."""
+    lib = native_lib
+    args = N.PagedAppendArgs(k=0x10000, v=0x10000, k_stride_token=256, k_stride_head=128, v_stride_token=256,
+                             v_stride_head=128, num_tokens=2)
+
+    def append(c, code, text, **kw):
+        a = N.PagedAppendArgs.from_buffer_copy(args)
+        for key, v in kw.items():
+            setattr(a, key, v)
+        assert lib.ypk_paged_append(C.byref(c), C.byref(a), None) == code
+        assert text in lib.ypk_last_error(None).decode(), lib.ypk_last_error(None)
+
+    assert lib.ypk_paged_append(None, C.byref(args), None) == N.ERR_INVALID
+    assert lib.ypk_paged_append(C.byref(c_cache()), None, None) == N.ERR_INVALID
+    append(c_cache(k=0), N.ERR_INVALID, "null cache")
+    append(c_cache(qo_indptr=None), N.ERR_INVALID, "row offsets")
+    append(c_cache(dtype=N.F32), N.ERR_UNSUPPORTED, "cache type")
+    append(c_cache(head_dim=96), N.ERR_UNSUPPORTED, "head_dim 96")
+    append(c_cache(page_size=0), N.ERR_INVALID, "0 tokens")
+    append(c_cache(num_requests=4097), N.ERR_UNSUPPORTED, "4097 requests")
+    append(c_cache(stride_token=260), N.ERR_INVALID, "16-byte")
+    append(c_cache(k=0x10008), N.ERR_INVALID, "16-byte")
+    append(c_cache(stride_head=0), N.ERR_INVALID, "overlap")
+    append(c_cache(), N.ERR_INVALID, "-1 tokens", num_tokens=-1)
+    append(c_cache(), N.ERR_INVALID, "come together", q=0x10000, num_q_heads=8)
+    append(c_cache(), N.ERR_INVALID, "7 query heads", q=0x10000, q_out=0x10000, num_q_heads=7)
+    append(c_cache(), N.ERR_INVALID, "cos and sin", cos=0x10000)
+    table = dict(cos=0x10000, sin=0x10000, table_dtype=N.BF16, max_positions=64, table_stride=128)
+    append(c_cache(), N.ERR_UNSUPPORTED, "24 rotated", rot_dim=24, **table)
+    append(c_cache(), N.ERR_UNSUPPORTED, "256 rotated", rot_dim=256, **table)
+    append(c_cache(), N.ERR_UNSUPPORTED, "table type", rot_dim=128, **dict(table, table_dtype=N.F16))
+    append(c_cache(), N.ERR_INVALID, "row stride 64", rot_dim=128, **dict(table, table_stride=64))
+    append(c_cache(), N.ERR_INVALID, "not 16-byte aligned", k=0x10002)
+    append(c_cache(), N.ERR_INVALID, "16-byte boundaries", k_stride_token=260)
+    a = N.PagedAppendArgs.from_buffer_copy(args)
+    a.num_tokens = 0
+    assert lib.ypk_paged_append(C.byref(c_cache()), C.byref(a), None) == N.YPK_OK     # nothing to do
+
+    def decode(c, code, text, **kw):
+        base = dict(q=0x10000, out=0x10000, workspace=0x10000, workspace_bytes=1 << 40, q_stride_token=1024,
+                    q_stride_group=512, q_stride_head=128, out_stride_token=1024, out_stride_group=512,
+                    out_stride_head=128, rows=2, num_q_heads=8, scale=0.1)
+        a = N.PagedDecodeArgs(**dict(base, **kw))
+        assert lib.ypk_paged_decode(C.byref(c), C.byref(a), None) == code
+        assert text in lib.ypk_last_error(None).decode(), lib.ypk_last_error(None)
+
+    decode(c_cache(), N.ERR_INVALID, "3 rows", rows=3)
+    decode(c_cache(), N.ERR_INVALID, "7 query heads", num_q_heads=7)
+    decode(c_cache(), N.ERR_INVALID, "window -1", window=-1)
+    decode(c_cache(), N.ERR_INVALID, "not finite", scale=float("nan"))
+    decode(c_cache(), N.ERR_INVALID, "not finite", scale=float("inf"))
+    decode(c_cache(), N.ERR_INVALID, "16-byte", q_stride_head=129)
+    decode(c_cache(), N.ERR_INVALID, "not 16-byte aligned", out=0x10002)
+    decode(c_cache(), N.ERR_INVALID, "null q", q=None)
+
+    def logprobs(code, text, **kw):
+        d = dict(dict(logits=0x10000, dtype=N.BF16, rows=2, vocab=100, ld=104, tokens=0x10000, top=2, lp=0x10000,
+                      ent=0x10000, tl=0x10000, tt=0x10000), **kw)
+        assert lib.ypk_token_logprobs(d["logits"], d["dtype"], d["rows"], d["vocab"], d["ld"], d["tokens"], d["top"],
+                                      d["lp"], d["ent"], d["tl"], d["tt"], None) == code
+        assert text in lib.ypk_last_error(None).decode(), lib.ypk_last_error(None)
+
+    logprobs(N.ERR_INVALID, "null", logits=None)
+    logprobs(N.ERR_INVALID, "null", ent=None)
+    logprobs(N.ERR_UNSUPPORTED, "type 955", dtype=N.I32)
+    logprobs(N.ERR_INVALID, "row stride 99", ld=99)
+    logprobs(N.ERR_INVALID, "vocabulary 0", vocab=0)
+    logprobs(N.ERR_UNSUPPORTED, "top_k 33", top=33)
+    logprobs(N.ERR_UNSUPPORTED, "top_k 5", top=5, vocab=4)
+    logprobs(N.ERR_INVALID, "top alternatives", tt=None)
+    logprobs(N.ERR_INVALID, "not aligned", logits=0x10001)
+    assert lib.ypk_token_logprobs(0x10000, N.BF16, 0, 100, 100, 0x10000, 0, 0x10000, 0x10000, None, None, None) == 0
+
+
+HARNESS = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <initializer_list>
+#include "paged_index.h"
+using namespace ypk;
+static void need(bool ok, const char *what) { if (!ok) { std::printf("%s\n", what); std::exit(1); } }
+int main() {
+  const int big = 0x7fffffff;
+  const int offsets[] = {-big - 1, -5, -1, 0, 1, 2, 3, 7, 8, 9, 100, big};
+  const int lasts[] = {-big - 1, -1, 0, 1, 5, 16, 17, big};
+  const int sizes[] = {1, 3, 16, 64, 4096, big};
+  for (int b : offsets) for (int e : offsets) for (int l : lasts) for (int ps : sizes) for (int n : {0, 1, 8, big}) {
+    const PagedRun r = paged_run(b, e, l, ps, n);
+    need(r.tokens >= 0, "negative length");
+    if (b == e) need(r.tokens == 0 && !r.broken, "empty slot");
+    if (r.broken) need(r.tokens == 0, "broken run has a length");
+    if (r.tokens == 0) continue;
+    // the first and the last position look up page numbers inside the list
+    need(r.first >= 0 && r.first < n, "first page number");
+    const int64_t last = r.first + (r.tokens - 1) / ps;
+    need(last >= r.first && last < n && last < e, "last page number");
+    for (int qo : offsets) for (int row : {0, 1, 5, big}) {
+      const int64_t p = paged_new_position(r, qo, row);
+      need(p < r.tokens, "new position behind the end");
+      if (row < qo) need(p == r.tokens - (int64_t(qo) - row), "new position");
+      else need(p == -1, "row behind the request");
+    }
+  }
+  // rows: inside the pool, at 64-bit offsets, or refused
+  for (int page : offsets) for (int pages : {1, 8, big}) for (int ps : {1, 3, 16, 64}) for (int64_t pos : {0L, 1L, 15L, 16L, 1000L, 1L << 40}) {
+    const int64_t st = 1024, sp = st * ps, row = paged_row(page, pages, pos, ps, sp, st);
+    if (page < 0 || page >= pages) need(row == -1, "page outside the pool");
+    else need(row == page * sp + (pos % ps) * st && row >= 0 && row + st <= int64_t(pages) * sp, "row");
+  }
+  std::puts("ok");
+}
+"""
+
+
+def test_paged_index_arithmetic_on_good_and_broken_tables(tmp_path):
+    """csrc/paged_index.h, the functions the kernels take every address from, compiled for the
+    host: no table, however broken, leads outside the page list or the pool."""
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    src = tmp_path / "walk.cpp"
+    src.write_text(HARNESS)
+    exe = tmp_path / "walk"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", os.path.join(ROOT, "yirage_b200", "csrc"), "-o", str(exe), str(src)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.strip() == "ok"
+
+
+def test_cached_prompts_that_cannot_enter_are_refused():
+    class Kernel:
+        max_num_batched_tokens, max_num_batched_requests, max_num_pages, page_size, max_seq_length = 8, 2, 4, 64, 100
+    rows = [torch.zeros(60, 2, 128, dtype=torch.bfloat16)]
+    state = {"meta": {"prompt_lengths": torch.tensor([70, 70, 70], dtype=torch.int32),
+                      "step": torch.zeros(3, dtype=torch.int32)},
+             "k_cache": torch.zeros(1, 4, 64, 2, 128, dtype=torch.bfloat16), "q_heads": 8}
+    for steps, what in (([60, 0], "one entry per request"), ([70, 0, 0], "less than its prompt"),
+                        ([-1, 0, 0], "less than its prompt"), ([0, 0, 60], "request 1 does not fit"),
+                        ([30, 20, 20], "60 rows|70 rows")):
+        with pytest.raises(ValueError, match=what):
+            llama.enter_cached_prompts(Kernel(), state, steps, rows, rows)
+    with pytest.raises(ValueError, match="1 layers"):
+        llama.enter_cached_prompts(Kernel(), state, [60, 0, 0], rows * 2, rows)

@@ -6,7 +6,7 @@ import yirage_b200 as _impl
 from yirage_b200 import *  # noqa: F401,F403
 from yirage_b200 import __version__  # noqa: F401
 
-for _name in ("core", "kernel", "lowering", "persistent_kernel", "speculative", "threadblock",
+for _name in ("core", "kernel", "lowering", "persistent_kernel", "serving", "speculative", "threadblock",
               "utils", "global_config", "version", "profiler_persistent"):
     try:
         _mod = __import__(f"yirage_b200.{_name}", fromlist=[_name])

@@ -42,6 +42,9 @@ F_LL_IN, F_LL_RES, F_LL_OUT, F_LL_PUSH, F_LL_OPT = 0x100, 0x200, 0x400, 0x800, 0
 F_TRIG_WIDE = 0x2000
 F_NORM_OUT, F_NORM_PRE = 0x8000, 0x10000
 
+# ypk_paged_cache.status
+PAGED_BAD_TABLE, PAGED_BAD_PAGE, PAGED_BAD_POSITION, PAGED_BAD_LENGTH = 1, 2, 4, 8
+
 NPTR, NINT, NFLT = 8, 16, 4
 
 
@@ -93,6 +96,43 @@ class Status(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("stride_page", C.c_int64), ("stride_token", C.c_int64), ("stride_head", C.c_int64),
+        ("indptr", C.c_void_p), ("indices", C.c_void_p), ("last_page_len", C.c_void_p),
+        ("qo_indptr", C.c_void_p), ("status", C.c_void_p),
+        ("dtype", C.c_int32), ("num_pages", C.c_int32), ("page_size", C.c_int32),
+        ("num_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("num_requests", C.c_int32),
+        ("num_indices", C.c_int32),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p),
+        ("cos", C.c_void_p), ("sin", C.c_void_p), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p),
+        ("k_stride_token", C.c_int64), ("k_stride_head", C.c_int64),
+        ("v_stride_token", C.c_int64), ("v_stride_head", C.c_int64),
+        ("q_stride_token", C.c_int64), ("q_stride_group", C.c_int64), ("q_stride_head", C.c_int64),
+        ("q_out_stride_token", C.c_int64), ("q_out_stride_group", C.c_int64),
+        ("q_out_stride_head", C.c_int64), ("table_stride", C.c_int64),
+        ("num_tokens", C.c_int32), ("num_q_heads", C.c_int32), ("rot_dim", C.c_int32),
+        ("max_positions", C.c_int32), ("table_dtype", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+class PagedDecodeArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("q_stride_token", C.c_int64), ("q_stride_group", C.c_int64), ("q_stride_head", C.c_int64),
+        ("out_stride_token", C.c_int64), ("out_stride_group", C.c_int64),
+        ("out_stride_head", C.c_int64),
+        ("rows", C.c_int32), ("num_q_heads", C.c_int32), ("window", C.c_int32), ("scale", C.c_float),
+    ]
+
+
 # Every symbol include/ypk.h declares: name -> (restype, argtypes)
 SYMBOLS = {
     "ypk_abi_version": (C.c_int, []),
@@ -122,6 +162,13 @@ SYMBOLS = {
     "ypk_adopt_batch": (C.c_int, [C.c_void_p, C.c_void_p]),
     "ypk_argmax_noalloc": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p,
                                      C.c_void_p]),
+    "ypk_paged_append": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "ypk_paged_decode": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedDecodeArgs), C.c_void_p]),
+    "ypk_paged_decode_workspace": (C.c_int, [C.POINTER(PagedCache), C.c_int32,
+                                             C.POINTER(C.c_uint64)]),
+    "ypk_token_logprobs": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int64,
+                                     C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                     C.c_void_p, C.c_void_p]),
     "ypk_transpose_16bit": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
 }
 

@@ -18,6 +18,7 @@
 #include "../../include/ypk.h"
 #include "argmax_noalloc.cuh"
 #include "megakernel.cuh"
+#include "op_common.h"
 #include "task_attention.cuh"   // kAttnRowFloats
 
 using namespace ypk;
@@ -109,6 +110,23 @@ int fail(ypk_handle *h, int code, const char *fmt, ...) {
   g_err = buf;
   return code;
 }
+
+}  // namespace
+
+namespace ypk {
+
+int op_fail(int code, const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return fail(nullptr, code, "%s", buf);
+}
+
+}  // namespace ypk
+
+namespace {
 
 #define CUDA_TRY(h, call)                                                              \
   do {                                                                                 \

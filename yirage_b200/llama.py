@@ -375,12 +375,65 @@ def build_decode_kernel(shape: LlamaShape, weights: Dict, *, tokens: torch.Tenso
                                     block_dim=(128, 1, 1))
     state = {"meta": meta, "k_cache": k_cache, "v_cache": v_cache, "cos": cos, "sin": sin,
              "lm_head": lm_head, "vocab_slice": (rank * vslice if vocab_parallel else 0, vslice),
-             "tensors": {"argmax_in": argmax_in, "attn_out": attn_out}}
+             "q_heads": hq, "tensors": {"argmax_in": argmax_in, "attn_out": attn_out}}
     if compile:
         # defer_connect: the caller exchanges the ranks' arena handles itself
         # (tensor_parallel.connect), e.g. after checking that every rank could build
         ypk.compile(dry_run=dry_run, defer_connect=defer_connect)
     return ypk, state
+
+
+def enter_cached_prompts(ypk: PersistentKernel, state: Dict, steps: List[int],
+                         keys: List[torch.Tensor], values: List[torch.Tensor]):
+    """Hand requests whose first tokens another engine has already run over to a kernel of
+    build_decode_kernel: after ypk.reset() and before the first launch.  Request r enters with
+    its first steps[r] tokens cached; keys[layer] / values[layer] [sum(steps), kv_heads,
+    head_dim] are their K / V rows in request order as the projections leave them (k after the
+    k norm of a model that has one, not yet rotated).  The rows go, rotated, to the pages that
+    the batcher is about to give the requests, and the step counters are set."""
+    from .serving import PagedKVCache
+    meta, kc = state["meta"], state["k_cache"]
+    dev, layers, page = kc.device, kc.shape[0], ypk.page_size
+    lengths = meta["prompt_lengths"].tolist()
+    if len(steps) != len(lengths) or any(
+            not 0 <= s <= max(0, min(n - 1, ypk.max_seq_length - 2)) for s, n in zip(steps, lengths)):
+        raise ValueError("steps: one entry per request, less than its prompt (its last token is the "
+                         "kernel's first input) and at most max_seq_length - 2")
+    if len(keys) != layers or len(values) != layers:
+        raise ValueError(f"{layers} layers of K and V rows are wanted")
+    if any(t.shape[0] != sum(steps) for t in (*keys, *values)):
+        raise ValueError(f"K and V must have {sum(steps)} rows")
+    # The first batch as the batcher will form it from the full page queue 0, 1, 2, ...: a
+    # request gets pages for its cached tokens and for its first chunk.
+    MT = ypk.max_num_batched_tokens
+    chunk = min(64, MT) if MT > 8 else min(8, 32 * kc.shape[3] // state["q_heads"])
+    indptr, pages, last, qo, taken, used = [0], [], [], [0], 0, 0
+    for r, (s, n) in enumerate(zip(steps, lengths)):
+        new = min(n - s, MT - taken, chunk) if n > s else min(1, MT - taken)
+        need = (s + new + page - 1) // page
+        enters = r < ypk.max_num_batched_requests and taken < MT and used + need <= ypk.max_num_pages
+        if not enters:
+            if any(steps[r:]):
+                raise ValueError(f"request {r} does not fit into the first batch: it cannot enter with cached tokens")
+            break
+        # the tables of the calls below: the request's pages as far as its cached tokens reach
+        pages += range(used, used + (s + page - 1) // page)
+        indptr.append(len(pages))
+        last.append((s - 1) % page + 1 if s else 0)
+        qo.append(qo[-1] + s)
+        taken += new
+        used += need
+    i32 = dict(dtype=torch.int32, device=dev)
+    tables = {"paged_kv_indptr_buffer": torch.tensor(indptr, **i32),
+              "paged_kv_indices_buffer": torch.tensor(pages, **i32),
+              "paged_kv_last_page_len_buffer": torch.tensor(last, **i32),
+              "qo_indptr_buffer": torch.tensor(qo, **i32)}
+    if pages:
+        for li in range(layers):
+            cache = PagedKVCache(kc[li], state["v_cache"][li], tables)
+            cache.append(keys[li], values[li], cos=state["cos"], sin=state["sin"])
+            cache.check()
+    meta["step"].copy_(torch.tensor(steps, **i32))
 
 
 class PrefillDecodePair:

@@ -630,6 +630,29 @@ class PersistentKernel:
         self._handle.read_tensor(t.guid, 0, out.data_ptr(), t.nbytes)
         return out
 
+    def token_logprobs(self, logits: DTensor, rows: int, tokens: Optional[torch.Tensor] = None,
+                       top_k: int = 0, valid_cols: Optional[int] = None):
+        """serving.token_logprobs over the first `rows` rows of a logits tensor of the graph as
+        the last launch left it, read in place: the log probabilities of what that iteration
+        sampled (`tokens`, by default the first `rows` output tokens), its entropy and
+        alternatives."""
+        from . import serving
+        if not self._is_compiled or self._dry:
+            raise RuntimeError("PersistentKernel is not compiled for a device")
+        if logits.num_dims != 2 or logits.dtype.code not in (N.F16, N.BF16, N.F32):
+            raise ValueError("logits must be a [tokens, columns] tensor of bf16, fp16 or fp32")
+        if not 0 <= rows <= logits.dim(0):
+            raise ValueError(f"{rows} rows of a tensor of {logits.dim(0)}")
+        vocab = logits.dim(1) if valid_cols is None else int(valid_cols)
+        if not 1 <= vocab <= logits.dim(1):
+            raise ValueError(f"valid_cols {vocab} of {logits.dim(1)} columns")
+        device = torch.device("cuda", self._handle.cfg.device)
+        if tokens is None:
+            tokens = self.meta_tensors["output_tokens"][:rows]
+        serving._check_tokens(tokens, rows, device)
+        ptr, _ = self._handle.tensor_ptr(logits.guid)
+        return serving._logprobs(ptr, logits.dtype.code, rows, vocab, logits.dim(1), tokens, top_k, device)
+
     def reset(self):
         """Back to the state right after compile(): step = 0, all pages free."""
         self._handle.reset()
