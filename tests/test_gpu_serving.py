@@ -170,6 +170,17 @@ def test_decode_split_over_long_lengths(hq, heads, lengths):
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)     # no order of arrival in it
 
 
+def test_decode_nan_in_a_seen_position_shows():
+    """A NaN among the seen K rows makes the heads that read it NaN, and no others."""
+    for n, at in ((100, 17), (5000, 4999), (1, 0)):
+        b = Batch([n, 50], seed=30)
+        b.k[b.where(0, torch.tensor([at], device="cuda"))[0], at % 64, 1, 5] = float("nan")
+        q = rnd(gen(31), 2, 8, 128)
+        out, lse = b.cache.decode(q, return_lse=True)
+        assert torch.isnan(out[0, 4:]).all() and torch.isnan(lse[0, 4:]).all()
+        assert torch.isfinite(out[0, :4]).all() and torch.isfinite(out[1]).all()
+
+
 def test_decode_many_requests():
     lengths = [(37 * i) % 190 for i in range(700)]
     run_decode(lengths, hq=4, heads=1, dim=64, page=16, seed=12)

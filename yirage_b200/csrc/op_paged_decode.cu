@@ -1,4 +1,30 @@
 // Attention of one new token per request over a paged cache (ypk_paged_decode).
+//
+//   out = sum_p w_p v_p / sum_p w_p,  w_p = 2^(y_p - m),  y_p = scale log2(e) q.k_p
+//
+// Every K and V row is read once, 2 len Hkv D elements in all, against 4 len Hq D operations: at
+// four query heads per K/V head that is 4 operations per byte, so memory bounds it and the
+// arithmetic only has to stay out of the way.  It goes to the tensor cores as mma m16n8k16 with
+// the sixteen cached tokens on the M side and the query heads of the group as the N side
+// (S^T = K Q^T, O^T = V^T P^T): a block of 16 tokens costs the same for one head as for eight.
+//
+// Work.  The unit is a block of 16 tokens of one (request, K/V head); all units of the call, in
+// that order, are cut into equal ranges, one per CTA and one CTA per SM, whatever the lengths
+// are: the lengths are read on the device, so the same captured launch serves every step.  A
+// (request, head) inside one range is finished there; of one that crosses ranges every CTA
+// leaves (m, sum, O) in the workspace and a second, dependent launch joins them in range order.
+// No atomics: the result does not depend on who comes first.
+//
+// Inside a CTA warp w takes the blocks w, w + 8, ...; each warp has its own ring of S blocks in
+// shared memory that it fills with 16-byte cp.async and reads with ldmatrix, so no barrier is
+// needed until a (request, head) ends and the warps' states are merged; the ring runs on
+// across that boundary.
+#include <math.h>
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
 #include "op_paged.h"
 
 namespace ypk {
@@ -11,92 +37,534 @@ struct DecodeArgs {
   float *lse;
   int64_t q_token, q_group, q_head, o_token, o_group, o_head;
   int rows, q_heads, group, window;
-  float scale;
+  int head_blocks;     // passes over a K/V head's rows: ceil(group / (8 NT))
+  int heads_per_pass;  // query heads of one pass, at most 8 NT
+  float scale_log2;
+  // workspace
+  int4 *desc;          // [workers] {request, pass, parts, 0} of the segment that starts a join here
+  float2 *part_ml;     // [workers][2][heads_per_pass] {m, sum}
+  float *part_o;       // [workers][2][heads_per_pass][D]
 };
 
-// One CTA of four warps per (request, query head); warp w takes positions w, w + 4, ..., a lane
-// holds D / 32 dimensions; running maximum and sum per warp, joined at the end.
-template <class T, int D>
-__global__ void __launch_bounds__(128) paged_decode_kernel(const DecodeArgs a) {
-  constexpr int E = D / 32;     // dimensions per lane: 2, 4 or 8
-  const int r = blockIdx.x, h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int g = h / a.group, i = h % a.group;
-  const PagedRun run = paged_run(a.c.indptr[r], a.c.indptr[r + 1], a.c.last[r], a.c.page_size, a.c.num_indices);
-  if (run.broken && threadIdx.x == 0) paged_flag(a.c, kPagedBadTable);
-  const uint32_t *qp = reinterpret_cast<const uint32_t *>(a.q + 2 * (r * a.q_token + g * a.q_group + i * a.q_head)) + lane * (E / 2);
-  float q[E], o[E];
-#pragma unroll
-  for (int e = 0; e < E / 2; ++e) {
-    const float2 f = T::widen(qp[e]);
-    q[2 * e] = f.x * a.scale;
-    q[2 * e + 1] = f.y * a.scale;
-    o[2 * e] = o[2 * e + 1] = 0.f;
+constexpr int kBlock = 16;             // tokens per unit of work
+// Units a CTA should have at least before the work is spread over more CTAs: two per warp.
+constexpr int kMinUnits = 16;
+
+template <class T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<OpBf16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<OpF16>(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  if (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+// 8 x 8 matrix of 16-bit values, one row per four lanes: transposed across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 bytes to shared memory; `valid` false writes zeros and reads nothing.
+__device__ __forceinline__ void copy16(uint32_t dst, const char *src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ int64_t range_start(int64_t total, int worker, int workers) {
+  return total * worker / workers;
+}
+
+// One (request, pass) as far as it lies in a CTA's range: blocks [ja, jb) of its nb.
+struct Segment {
+  int64_t left;     // units of the range behind this segment
+  int r, pass, ja, jb, nb, b0, len, lo, first;
+};
+
+template <int NW, int D, int NT, int S>
+struct DecodeShape {
+  static constexpr int kRowBytes = 2 * D;
+  static constexpr int kTile = kBlock * kRowBytes;     // one of K, V
+  static constexpr int kRing = NW * S * 2 * kTile;
+  static constexpr int kHeads = 8 * NT;
+  // warps' states at a merge: m and sum, then O
+  static int merge_bytes(int heads) { return NW * heads * (8 + D * 4); }
+  static int bytes(int heads, int rows) { return kRing + merge_bytes(heads) + NW * S * 4 + rows * 8; }
+};
+
+template <class T, int NW, int D, int NT, int S>
+__global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_constant__ DecodeArgs a) {
+  using Shape = DecodeShape<NW, D, NT, S>;
+  constexpr int kThreads = NW * 32;
+  constexpr int kChunks = D / 8;                  // 16-byte chunks per row
+  // P in fp16 keeps a few powers of two of head room below: weights down to 2^-31 of the largest
+  // survive (bf16 has fp32's range)
+  constexpr float kShift = std::is_same<T, OpF16>::value ? 7.f : 0.f;
+  extern __shared__ __align__(128) char smem[];
+  __shared__ int64_t s_warp_total[NW];
+  __shared__ Segment s_start;
+
+  // the joining launch may begin to set itself up; it waits for this grid before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int heads = a.heads_per_pass;
+  char *ring = smem;
+  float2 *m_ml = reinterpret_cast<float2 *>(smem + Shape::kRing);          // [NW][heads]
+  float *m_o = reinterpret_cast<float *>(m_ml + NW * heads);               // [NW][heads][D]
+  int *s_mask = reinterpret_cast<int *>(m_o + NW * heads * D);             // [NW][S]
+  int *s_first = s_mask + NW * S;                                          // [rows]
+  int *s_len = s_first + a.rows;                                           // [rows]
+
+  // ---- the batch: lengths, this CTA's range, where in the batch it begins
+  const int passes = a.c.kv_heads * a.head_blocks;
+  const int per = (a.rows + kThreads - 1) / kThreads;
+  const auto blocks_of = [&](int len) {
+    const int lo = a.window > 0 && len > a.window ? len - a.window : 0;
+    return (len + kBlock - 1) / kBlock - lo / kBlock;
+  };
+  int64_t mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int r = tid * per + i;
+    if (r >= a.rows) break;
+    const PagedRun run = paged_run(a.c.indptr[r], a.c.indptr[r + 1], a.c.last[r], a.c.page_size, a.c.num_indices);
+    if (run.broken && blockIdx.x == 0) paged_flag(a.c, kPagedBadTable);
+    s_first[r] = int(run.first);
+    s_len[r] = int(run.tokens);
+    mine += int64_t(blocks_of(int(run.tokens))) * passes;
   }
-  float m = -INFINITY, l = 0.f;
-  const int64_t first = a.window > 0 && run.tokens > a.window ? run.tokens - a.window : 0;
-  for (int64_t p = first + warp; p < run.tokens; p += 4) {
-    const int64_t row = paged_row(a.c.indices[run.first + p / a.c.page_size], a.c.num_pages, p, a.c.page_size,
-                                  a.c.stride_page, a.c.stride_token);
-    if (row < 0) {
-      if (lane == 0) paged_flag(a.c, kPagedBadPage);
-      continue;
-    }
-    const uint32_t *kp = reinterpret_cast<const uint32_t *>(a.c.k + 2 * (row + g * a.c.stride_head)) + lane * (E / 2);
-    const uint32_t *vp = reinterpret_cast<const uint32_t *>(a.c.v + 2 * (row + g * a.c.stride_head)) + lane * (E / 2);
-    float s = 0.f;
+  int64_t before = mine;            // inclusive scan over the threads
 #pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      const float2 f = T::widen(kp[e]);
-      s += q[2 * e] * f.x + q[2 * e + 1] * f.y;
-    }
-#pragma unroll
-    for (int x = 16; x; x /= 2) s += __shfl_xor_sync(~0u, s, x);
-    const float top = fmaxf(m, s);
-    const float keep = __expf(m - top), w = __expf(s - top);
-    m = top;
-    l = l * keep + w;
-#pragma unroll
-    for (int e = 0; e < E / 2; ++e) {
-      const float2 f = T::widen(vp[e]);
-      o[2 * e] = o[2 * e] * keep + w * f.x;
-      o[2 * e + 1] = o[2 * e + 1] * keep + w * f.y;
-    }
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t x = __shfl_up_sync(~0u, before, o);
+    if (lane >= o) before += x;
   }
-  __shared__ float sm[4], sl[4], so[4][D];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) so[warp][lane * E + e] = o[e];
+  if (lane == 31) s_warp_total[warp] = before;
   __syncthreads();
-  float top = -INFINITY, total = 0.f;
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w]);
-  float f[4];
-  for (int w = 0; w < 4; ++w) {
-    f[w] = sm[w] == -INFINITY ? 0.f : __expf(sm[w] - top);
-    total += f[w] * sl[w];
+  int64_t total = 0;
+  before -= mine;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) before += s_warp_total[w];
+    total += s_warp_total[w];
   }
-  const float inv = total > 0.f ? 1.f / total : 0.f;
-  uint32_t *op = reinterpret_cast<uint32_t *>(a.out + 2 * (r * a.o_token + g * a.o_group + i * a.o_head));
-  for (int d = threadIdx.x; d < D / 2; d += 128) {
-    float x = 0.f, y = 0.f;
-    for (int w = 0; w < 4; ++w) {
-      x += f[w] * so[w][2 * d];
-      y += f[w] * so[w][2 * d + 1];
+  const int64_t want = total / kMinUnits;
+  const int workers = want < 1 ? 1 : want < int64_t(gridDim.x) ? int(want) : int(gridDim.x);
+  const bool works = total > 0 && int(blockIdx.x) < workers;
+  const int64_t u0 = works ? range_start(total, blockIdx.x, workers) : 0;
+  const int64_t u1 = works ? range_start(total, blockIdx.x + 1, workers) : 0;
+  const auto fill = [&](Segment &s) {   // what follows from the request
+    s.first = s_first[s.r];
+    s.len = s_len[s.r];
+    s.lo = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
+    s.b0 = s.lo / kBlock;
+    s.nb = blocks_of(s.len);
+  };
+  if (works && u0 >= before && u0 < before + mine) {
+    int64_t off = u0 - before;
+    Segment s;
+    for (s.r = tid * per;; ++s.r) {
+      fill(s);
+      if (off < int64_t(s.nb) * passes) break;
+      off -= int64_t(s.nb) * passes;
     }
-    op[d] = T::round2(x * inv, y * inv);
+    s.pass = int(off / s.nb);
+    s.ja = int(off % s.nb);
+    s.jb = int(min(int64_t(s.nb), s.ja + (u1 - u0)));
+    s.left = (u1 - u0) - (s.jb - s.ja);
+    s_start = s;
   }
-  if (a.lse && threadIdx.x == 0) a.lse[int64_t(r) * a.q_heads + h] = total > 0.f ? top + logf(total) : -INFINITY;
+  if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+  // requests without positions: nobody's range
+  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    // (s_len of r was written by this CTA before the barrier above)
+    if (s_len[r] != 0) continue;
+    for (int i = tid; i < a.q_heads * (D / 8); i += kThreads) {
+      const int h = i / (D / 8);
+      *reinterpret_cast<uint4 *>(a.out + 2 * (r * a.o_token + (h / a.group) * a.o_group + (h % a.group) * a.o_head) +
+                                 16 * (i % (D / 8))) = make_uint4(0, 0, 0, 0);
+    }
+    if (a.lse)
+      for (int h = tid; h < a.q_heads; h += kThreads) a.lse[int64_t(r) * a.q_heads + h] = -INFINITY;
+  }
+  __syncthreads();
+  if (!works) return;
+
+  const auto next_segment = [&](Segment &s) {   // only while s.left > 0
+    if (++s.pass == passes) {
+      s.pass = 0;
+      do ++s.r;
+      while (s_len[s.r] == 0);
+      fill(s);
+    }
+    s.ja = 0;
+    s.jb = int(min(int64_t(s.nb), s.left));
+    s.left -= s.jb;
+  };
+
+  // ---- filling the ring: this warp's blocks one after the other, across segments
+  char *my_ring = ring + warp * (S * 2 * Shape::kTile);
+  const uint32_t my_ring32 = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
+  Segment fs = s_start;
+  int fj = fs.ja + warp;
+  int page = 0;                // of this lane's row (lane % 16) in the block at the cursor
+  bool more = true;            // the cursor stands on a block
+  const auto settle = [&]() {  // move the cursor onto a block, fetch its page numbers
+    while (fj >= fs.jb) {
+      if (fs.left == 0) {
+        more = false;
+        return;
+      }
+      next_segment(fs);
+      fj = warp;
+    }
+    const int pos = (fs.b0 + fj) * kBlock + lane % kBlock;
+    page = pos < fs.len && pos >= fs.lo ? __ldg(a.c.indices + fs.first + pos / a.c.page_size) : -1;
+  };
+  int fstage = 0;
+  const auto issue = [&]() {
+    if (more) {
+      const int pos = (fs.b0 + fj) * kBlock + lane % kBlock;
+      const bool inside = pos < fs.len && pos >= fs.lo;
+      int64_t row = inside ? paged_row(page, a.c.num_pages, pos, a.c.page_size, a.c.stride_page, a.c.stride_token) : -1;
+      if (inside && row < 0) paged_flag(a.c, kPagedBadPage);
+      const unsigned mask = __ballot_sync(~0u, row >= 0) & 0xffffu;
+      if (lane == 0) s_mask[warp * S + fstage] = int(mask);
+      if (row >= 0) row = 2 * (row + (fs.pass / a.head_blocks) * a.c.stride_head);
+      const uint32_t dst = my_ring32 + fstage * 2 * Shape::kTile;
+#pragma unroll
+      for (int i = 0; i < kBlock * kChunks / 32; ++i) {
+        const int t = i * 32 + lane, rr = t / kChunks, ch = t % kChunks;
+        const int64_t at = __shfl_sync(~0u, row, rr);
+        const bool valid = at >= 0;
+        const int64_t src = valid ? at + ch * 16 : 0;
+        const uint32_t to = dst + rr * Shape::kRowBytes + ((ch ^ (rr & 7)) * 16);
+        copy16(to, a.c.k + src, valid);
+        copy16(to + Shape::kTile, a.c.v + src, valid);
+      }
+      fstage = fstage + 1 == S ? 0 : fstage + 1;
+      fj += NW;
+      settle();
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  settle();
+#pragma unroll
+  for (int s = 0; s < S - 1; ++s) issue();
+
+  // ---- consuming
+  int stage = 0;
+  Segment cs = s_start;
+  for (;;) {
+    const int kv = cs.pass / a.head_blocks, h0 = (cs.pass % a.head_blocks) * heads;
+    const int live = min(heads, a.group - h0);        // query heads of this pass
+    uint32_t qf[NT][D / 16][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int h = n * 8 + lane / 4;
+      const char *qp = a.q + 2 * (cs.r * a.q_token + kv * a.q_group + (h0 + h) * a.q_head) + (lane % 4) * 4;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        qf[n][ks][0] = h < live ? *reinterpret_cast<const uint32_t *>(qp + ks * 32) : 0u;
+        qf[n][ks][1] = h < live ? *reinterpret_cast<const uint32_t *>(qp + ks * 32 + 16) : 0u;
+      }
+    }
+    float o[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
+    }
+    for (int j = cs.ja + warp; j < cs.jb; j += NW) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+      __syncwarp();
+      issue();         // into the stage that the previous block has left
+      const uint32_t kt = my_ring32 + stage * 2 * Shape::kTile, vt = kt + Shape::kTile;
+      const int mask = s_mask[warp * S + stage];
+      stage = stage + 1 == S ? 0 : stage + 1;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t af[4];
+        const int row = (lane / 8 % 2) * 8 + lane % 8, ch = ks * 2 + lane / 16;
+        ldmatrix4<false>(af, kt + row * Shape::kRowBytes + ((ch ^ (row & 7)) * 16));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816<T>(s[n], af, qf[n][ks][0], qf[n][ks][1]);
+      }
+      const bool v0 = (mask >> (lane / 4)) & 1, v1 = (mask >> (lane / 4 + 8)) & 1;
+      bool grows = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        s[n][0] = v0 ? s[n][0] * a.scale_log2 : -INFINITY;
+        s[n][1] = v0 ? s[n][1] * a.scale_log2 : -INFINITY;
+        s[n][2] = v1 ? s[n][2] * a.scale_log2 : -INFINITY;
+        s[n][3] = v1 ? s[n][3] * a.scale_log2 : -INFINITY;
+        // weights up to 2^8 over the reference are let through: the reference moves rarely
+        grows |= fmaxf(s[n][0], s[n][2]) > m[n][0] + 8.f || fmaxf(s[n][1], s[n][3]) > m[n][1] + 8.f;
+      }
+      if (__any_sync(~0u, grows)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float top = fmaxf(s[n][c], s[n][c + 2]);
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+            top = fmaxf(top, m[n][c]);
+            const float keep = m[n][c] == -INFINITY ? 0.f : exp2_fast(m[n][c] - top);
+            m[n][c] = top;
+            l[n][c] *= keep;
+#pragma unroll
+            for (int d = 0; d < D / 16; ++d) {
+              o[n][d][c] *= keep;
+              o[n][d][c + 2] *= keep;
+            }
+          }
+      }
+      uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float p[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float ref = m[n][c & 1] == -INFINITY ? 0.f : m[n][c & 1];
+          p[c] = exp2_fast(s[n][c] - ref + kShift);
+        }
+        l[n][0] += p[0] + p[2];
+        l[n][1] += p[1] + p[3];
+        // The weights go into the product as two 16-bit parts, 16 bits of them in all: one part
+        // alone would err as much as the rounding of the result itself.
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t h = T::round2(p[2 * c], p[2 * c + 1]);
+          const float2 f = T::widen(h);
+          hi[n][c] = transpose8(h);
+          lo[n][c] = transpose8(T::round2(p[2 * c] - f.x, p[2 * c + 1] - f.y));
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        uint32_t af[4];
+        const int row = (lane / 16) * 8 + lane % 8, ch = d * 2 + lane / 8 % 2;
+        ldmatrix4<true>(af, vt + row * Shape::kRowBytes + ((ch ^ (row & 7)) * 16));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816<T>(o[n][d], af, hi[n][0], hi[n][1]);
+          mma16816<T>(o[n][d], af, lo[n][0], lo[n][1]);
+        }
+      }
+    }
+    // ---- merge the warps
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) l[n][c] += __shfl_xor_sync(~0u, l[n][c], x);
+        const int h = n * 8 + (lane % 4) * 2 + c;
+        if (h < live) {
+          if (lane < 4) m_ml[warp * heads + h] = make_float2(m[n][c], l[n][c]);
+          float *po = m_o + (warp * heads + h) * D + lane / 4;
+#pragma unroll
+          for (int d = 0; d < D / 16; ++d) {
+            po[d * 16] = o[n][d][c];
+            po[d * 16 + 8] = o[n][d][c + 2];
+          }
+        }
+      }
+    __syncthreads();
+    const bool whole = cs.ja == 0 && cs.jb == cs.nb;
+    const int slot = 2 * blockIdx.x + (cs.ja == 0);    // 1: the range that begins the segment
+    for (int i = tid; i < live * (D / 4); i += kThreads) {
+      const int h = i / (D / 4), d = i % (D / 4) * 4;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) top = fmaxf(top, m_ml[w * heads + h].x);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float2 ml = m_ml[w * heads + h];
+        const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);   // (a NaN sum stays one)
+        const float4 y = *reinterpret_cast<const float4 *>(m_o + (w * heads + h) * D + d);
+        sum += f * ml.y;
+        x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+      }
+      if (whole) {
+        const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+        const uint2 v = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
+        *reinterpret_cast<uint2 *>(a.out + 2 * (cs.r * a.o_token + kv * a.o_group + (h0 + h) * a.o_head + d)) = v;
+        if (a.lse && d == 0)
+          a.lse[int64_t(cs.r) * a.q_heads + kv * a.group + h0 + h] =
+              sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.69314718055994531f;
+      } else {
+        *reinterpret_cast<float4 *>(a.part_o + (int64_t(slot) * heads + h) * D + d) = x;
+        if (d == 0) a.part_ml[int64_t(slot) * heads + h] = make_float2(top, sum);
+      }
+    }
+    if (!whole && cs.ja == 0 && tid == 0) {
+      // this range begins the segment: tell the joining launch how many ranges it runs through
+      const int64_t end = u1 + (cs.nb - cs.jb);       // one past the segment's last unit
+      int last = int(min(int64_t(workers - 1), (end - 1) * workers / total));
+      while (last + 1 < workers && range_start(total, last + 1, workers) <= end - 1) ++last;
+      while (range_start(total, last, workers) > end - 1) --last;
+      a.desc[blockIdx.x] = make_int4(cs.r, cs.pass, last - int(blockIdx.x) + 1, 0);
+    }
+    if (cs.left == 0) break;
+    __syncthreads();      // the merge area is free again
+    next_segment(cs);
+  }
+}
+
+// Joins the parts of the segment that begins in worker blockIdx.x's range, for query head
+// blockIdx.y of the pass: parts of workers x (slot 1), x + 1, ... (slot 0).
+template <class T, int D>
+__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ DecodeArgs a) {
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;      // threads per row, rows at a time
+  constexpr float kShift = std::is_same<T, OpF16>::value ? 7.f : 0.f;
+  __shared__ float s_red[8];
+  __shared__ float s_sum[kGroups];
+  __shared__ float4 s_o[kGroups][kLanes];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 desc = a.desc[blockIdx.x];
+  const int parts = desc.z, heads = a.heads_per_pass, h = blockIdx.y;
+  const int kv = desc.y / a.head_blocks, h0 = (desc.y % a.head_blocks) * heads;
+  if (parts == 0 || h0 + h >= a.group) return;
+  const auto row_of = [&](int i) { return (int64_t(2) * (blockIdx.x + i) + (i == 0)) * heads + h; };
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < parts; i += 256) top = fmaxf(top, a.part_ml[row_of(i)].x);
+#pragma unroll
+  for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+  if (threadIdx.x % 32 == 0) s_red[threadIdx.x / 32] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, s_red[w]);
+  const int g = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+#pragma unroll 8
+  for (int i = g; i < parts; i += kGroups) {
+    const float2 ml = a.part_ml[row_of(i)];
+    const float4 y = *reinterpret_cast<const float4 *>(a.part_o + row_of(i) * D + d * 4);
+    const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);
+    sum += f * ml.y;
+    x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+  }
+  s_o[g][d] = x;
+  if (d == 0) s_sum[g] = sum;
+  __syncthreads();
+  if (g != 0) return;
+#pragma unroll
+  for (int i = 1; i < kGroups; ++i) {
+    const float4 y = s_o[i][d];
+    sum += s_sum[i];
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+  }
+  const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+  const uint2 v = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
+  *reinterpret_cast<uint2 *>(a.out + 2 * (desc.x * a.o_token + kv * a.o_group + (h0 + h) * a.o_head + d * 4)) = v;
+  if (a.lse && d == 0)
+    a.lse[int64_t(desc.x) * a.q_heads + kv * a.group + h0 + h] =
+        sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.69314718055994531f;
+}
+
+// Query heads per pass: eight fill one n-tile of the product.  Sixteen (two n-tiles) read the rows
+// once for groups of 9 to 16; at D = 256 the second tile's accumulators do not fit the registers.
+int n_tiles(int head_dim, int group) { return head_dim <= 128 && group > 8 ? 2 : 1; }
+
+int pass_heads(int head_dim, int group) { return std::min(group, 8 * n_tiles(head_dim, group)); }
+
+struct DeviceInfo {
+  int device, sms;
+};
+
+// SM count of the current device, asked for once per device.
+int device_info(DeviceInfo *d) {
+  static std::atomic<int> sms_of[64];
+  cudaError_t e = cudaGetDevice(&d->device);
+  if (e != cudaSuccess || d->device < 0 || d->device >= 64)
+    return op_fail(YPK_ERR_CUDA, "paged_decode: no current device (%s)", cudaGetErrorString(e));
+  d->sms = sms_of[d->device].load(std::memory_order_relaxed);
+  if (!d->sms) {
+    e = cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, d->device);
+    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: SM count: %s", cudaGetErrorString(e));
+    sms_of[d->device].store(d->sms, std::memory_order_relaxed);
+  }
+  return YPK_OK;
+}
+
+uint64_t workspace_bytes(int workers, int heads, int head_dim) {
+  return uint64_t(workers) * (16 + 2 * uint64_t(heads) * (8 + 4 * uint64_t(head_dim)));
+}
+
+constexpr int kMaxShared = 232448 - 1024;   // opt-in limit of a block, less the static part
+
+template <class T, int NW, int D, int NT, int S>
+int launch_shape(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
+  using Shape = DecodeShape<NW, D, NT, S>;
+  static std::atomic<uint64_t> ready{0};      // devices whose limit has been raised
+  auto *kernel = paged_decode_kernel<T, NW, D, NT, S>;
+  if (!(ready.load(std::memory_order_relaxed) >> dev.device & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
+    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: shared memory: %s", cudaGetErrorString(e));
+    ready.fetch_or(uint64_t(1) << dev.device, std::memory_order_relaxed);
+  }
+  kernel<<<dev.sms, NW * 32, Shape::bytes(a.heads_per_pass, a.rows), st>>>(a);
+  if (int rc = op_launched("paged_decode")) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(dev.sms, a.heads_per_pass);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a);
+  if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: joining launch: %s", cudaGetErrorString(e));
+  return YPK_OK;
+}
+
+// Ring depth: three blocks per warp; two where the merge area of sixteen heads or the tables of
+// thousands of requests need the room.
+template <class T, int NW, int D, int NT>
+int launch_ring(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
+  if (DecodeShape<NW, D, NT, 3>::bytes(a.heads_per_pass, a.rows) <= kMaxShared)
+    return launch_shape<T, NW, D, NT, 3>(a, dev, st);
+  return launch_shape<T, NW, D, NT, 2>(a, dev, st);
 }
 
 template <class T>
-int launch_decode(int head_dim, const DecodeArgs &a, cudaStream_t st) {
-  const dim3 grid(a.rows, a.q_heads);
-  if (head_dim == 64) paged_decode_kernel<T, 64><<<grid, 128, 0, st>>>(a);
-  else if (head_dim == 128) paged_decode_kernel<T, 128><<<grid, 128, 0, st>>>(a);
-  else paged_decode_kernel<T, 256><<<grid, 128, 0, st>>>(a);
-  return op_launched("paged_decode");
+int launch_decode(int head_dim, const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
+  const bool two = n_tiles(head_dim, a.group) == 2;
+  if (head_dim == 64) return two ? launch_ring<T, 8, 64, 2>(a, dev, st) : launch_ring<T, 8, 64, 1>(a, dev, st);
+  if (head_dim == 128) return two ? launch_ring<T, 8, 128, 2>(a, dev, st) : launch_ring<T, 8, 128, 1>(a, dev, st);
+  return launch_ring<T, 4, 256, 1>(a, dev, st);
 }
 
 int check_heads(const ypk_paged_cache *cache, int q_heads) {
@@ -114,7 +582,9 @@ extern "C" int ypk_paged_decode_workspace(const ypk_paged_cache *cache, int32_t 
   if (int rc = paged_check("paged_decode", cache, false)) return rc;
   if (int rc = check_heads(cache, num_q_heads)) return rc;
   if (!bytes) return op_fail(YPK_ERR_INVALID, "paged_decode: null size");
-  *bytes = 16;
+  DeviceInfo dev;
+  if (int rc = device_info(&dev)) return rc;
+  *bytes = workspace_bytes(dev.sms, pass_heads(cache->head_dim, num_q_heads / cache->num_kv_heads), cache->head_dim);
   return YPK_OK;
 }
 
@@ -127,18 +597,14 @@ extern "C" int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_de
   if (p->rows == 0) return YPK_OK;
   if (!p->q || !p->out) return op_fail(YPK_ERR_INVALID, "paged_decode: null q or out");
   if (p->window < 0) return op_fail(YPK_ERR_INVALID, "paged_decode: window %d", p->window);
-  if (!(p->scale == p->scale) || p->scale - p->scale != 0.f)
-    return op_fail(YPK_ERR_INVALID, "paged_decode: scale is not finite");
+  if (!(fabsf(p->scale) <= 1e30f)) return op_fail(YPK_ERR_INVALID, "paged_decode: scale is not finite");
   for (int64_t s : {p->q_stride_token, p->q_stride_group, p->q_stride_head, p->out_stride_token,
                     p->out_stride_group, p->out_stride_head})
     if (s < 0 || s % 8) return op_fail(YPK_ERR_INVALID, "paged_decode: rows must start on 16-byte boundaries");
   if (!op_aligned16(p->q) || !op_aligned16(p->out) || !op_aligned16(p->workspace))
     return op_fail(YPK_ERR_INVALID, "paged_decode: an operand is not 16-byte aligned");
-  uint64_t need = 0;
-  if (int rc = ypk_paged_decode_workspace(cache, p->num_q_heads, &need)) return rc;
-  if (!p->workspace || p->workspace_bytes < need)
-    return op_fail(YPK_ERR_INVALID, "paged_decode: workspace of %llu bytes, %llu needed",
-                   (unsigned long long)(p->workspace ? p->workspace_bytes : 0), (unsigned long long)need);
+  DeviceInfo dev;
+  if (int rc = device_info(&dev)) return rc;
   DecodeArgs a;
   a.c = paged_view(cache);
   a.q = static_cast<const char *>(p->q);
@@ -150,8 +616,18 @@ extern "C" int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_de
   a.q_heads = p->num_q_heads;
   a.group = p->num_q_heads / cache->num_kv_heads;
   a.window = p->window;
-  a.scale = p->scale;
+  a.heads_per_pass = pass_heads(cache->head_dim, a.group);
+  a.head_blocks = (a.group + a.heads_per_pass - 1) / a.heads_per_pass;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  const uint64_t need = workspace_bytes(dev.sms, a.heads_per_pass, cache->head_dim);
+  if (!p->workspace || p->workspace_bytes < need)
+    return op_fail(YPK_ERR_INVALID, "paged_decode: workspace of %llu bytes, %llu needed",
+                   (unsigned long long)(p->workspace ? p->workspace_bytes : 0), (unsigned long long)need);
+  char *w = static_cast<char *>(p->workspace);
+  a.desc = reinterpret_cast<int4 *>(w);
+  a.part_o = reinterpret_cast<float *>(w + 16 * uint64_t(dev.sms));
+  a.part_ml = reinterpret_cast<float2 *>(a.part_o + 2 * uint64_t(dev.sms) * a.heads_per_pass * cache->head_dim);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return cache->dtype == YPK_BF16 ? launch_decode<OpBf16>(cache->head_dim, a, st)
-                                  : launch_decode<OpF16>(cache->head_dim, a, st);
+  return cache->dtype == YPK_BF16 ? launch_decode<OpBf16>(cache->head_dim, a, dev, st)
+                                  : launch_decode<OpF16>(cache->head_dim, a, dev, st);
 }

@@ -23,6 +23,9 @@ constexpr int kPagedBadPage = 2;       // a page number outside the pool
 constexpr int kPagedBadPosition = 4;   // a position outside the rotary tables
 constexpr int kPagedBadLength = 8;     // more new tokens than the request is long
 
+// Longest request: positions, and positions rounded up to a block, fit 32 bits.
+constexpr int64_t kPagedMaxTokens = 0x7fffff00;
+
 // The run of one request in the list of page numbers, and its length in tokens.
 struct PagedRun {
   int64_t first;    // index of its first page number
@@ -38,6 +41,10 @@ YPK_HD PagedRun paged_run(int begin, int end, int last_page_len, int page_size, 
     return r;
   }
   r.tokens = int64_t(end - begin - 1) * page_size + last_page_len;
+  if (r.tokens > kPagedMaxTokens) {                 // no memory holds it: the table is broken
+    r.tokens = 0;
+    r.broken = true;
+  }
   return r;
 }
 
