@@ -538,6 +538,24 @@ def test_logprobs_sorted_rows(rising):
         check_logprobs(x.to(BF16), torch.full((rows,), n // 2, device="cuda"), 7)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows", [1, 700])
+def test_logprobs_high_columns_crowded(dtype, rows):
+    """Thousands of high values in the columns of a few threads, equal or not: more than the list of
+    candidates holds."""
+    g = gen(8)
+    n, width = 60000, 8 if dtype == BF16 else 4
+    col = torch.arange(n, device="cuda")
+    for block in (512, 64):
+        crowd = ((col // width) % block) % 24 == 5
+        x = rnd(g, rows, n, dtype=dtype)
+        t = torch.randint(0, n, (rows,), generator=g, device="cuda")
+        check_logprobs(torch.where(crowd, x + 9, x), t, 32)
+        check_logprobs(torch.where(crowd, torch.full_like(x, 9), x), t, 32)
+        few = torch.where(col % 9001 == 77, x + 20, torch.full_like(x, float("-inf")))
+        check_logprobs(few, t, 20)                  # fewer columns than alternatives
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 def test_logprobs_masked_rows(dtype):
     g = gen(3)
