@@ -646,12 +646,11 @@ class PersistentKernel:
         vocab = logits.dim(1) if valid_cols is None else int(valid_cols)
         if not 1 <= vocab <= logits.dim(1):
             raise ValueError(f"valid_cols {vocab} of {logits.dim(1)} columns")
-        device = torch.device("cuda", self._handle.cfg.device)
         if tokens is None:
             tokens = self.meta_tensors["output_tokens"][:rows]
-        serving._check_tokens(tokens, rows, device)
         ptr, _ = self._handle.tensor_ptr(logits.guid)
-        return serving._logprobs(ptr, logits.dtype.code, rows, vocab, logits.dim(1), tokens, top_k, device)
+        return serving.TokenLogprobs._make(serving._load().logprobs_at(
+            ptr, logits.dtype.code, rows, vocab, logits.dim(1), tokens, top_k, self._handle.cfg.device))
 
     def reset(self):
         """Back to the state right after compile(): step = 0, all pages free."""
