@@ -19,6 +19,7 @@
 // shared memory that it fills with 16-byte cp.async and reads with ldmatrix, so no barrier is
 // needed until a (request, head) ends and the warps' states are merged; the ring runs on
 // across that boundary.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include <algorithm>
@@ -26,6 +27,8 @@
 #include <type_traits>
 
 #include "op_paged.h"
+
+namespace cg = cooperative_groups;
 
 namespace ypk {
 namespace {
@@ -37,11 +40,14 @@ struct DecodeArgs {
   float *lse;
   int64_t q_token, q_group, q_head, o_token, o_group, o_head;
   int rows, q_heads, group, window;
+  int ctas;            // per (request, pass) where clusters are used
   int head_blocks;     // passes over a K/V head's rows: ceil(group / (8 NT))
   int heads_per_pass;  // query heads of one pass, at most 8 NT
   float scale_log2;
   // workspace
-  int4 *desc;          // [workers] {request, pass, parts, 0} of the segment that starts a join here
+  int by_segment;      // the segments are few: desc is indexed by segment, not by worker
+  int4 *desc;          // {request, pass, parts, worker}: a segment in several parts, the first that
+                       // worker's; parts = 0: nothing to join
   float2 *part_ml;     // [workers][2][heads_per_pass] {m, sum}
   float *part_o;       // [workers][2][heads_per_pass][D]
 };
@@ -49,6 +55,11 @@ struct DecodeArgs {
 constexpr int kBlock = 16;             // tokens per unit of work
 // Units a CTA should have at least before the work is spread over more CTAs: two per warp.
 constexpr int kMinUnits = 16;
+constexpr int kAlignUnits = 80;
+// Segments of at most this many blocks are not cut: they go whole to the range that holds the
+// larger part of them.
+constexpr int kSnapUnits = 16;
+constexpr int kMaxCluster = 8;
 
 template <class T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -93,9 +104,24 @@ __device__ __forceinline__ void copy16(uint32_t dst, const char *src, bool valid
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 
-__device__ __forceinline__ int64_t range_start(int64_t total, int worker, int workers) {
-  return total * worker / workers;
+// 64-bit division is a subroutine of a hundred instructions; the numbers here nearly always fit 32.
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+  return (a | b) >> 32 ? a / b : int64_t(uint32_t(a) / uint32_t(b));
 }
+
+// The units of a call cut into equal ranges: worker w's begins at floor(total w / workers).
+struct Ranges {
+  int64_t total, each;
+  int workers, more;       // total = each workers + more
+  __device__ __forceinline__ int64_t start(int w) const {
+    return each * w + uint32_t(more) * uint32_t(w) / uint32_t(workers);
+  }
+  __device__ __forceinline__ int owner(int64_t u) const {   // the worker whose range u lies in
+    int w = int(min(int64_t(workers - 1), divide(u, each)));   // (each <= a range: not too low)
+    while (start(w) > u) --w;
+    return w;
+  }
+};
 
 // One (request, pass) as far as it lies in a CTA's range: blocks [ja, jb) of its nb.
 struct Segment {
@@ -108,13 +134,14 @@ struct DecodeShape {
   static constexpr int kRowBytes = 2 * D;
   static constexpr int kTile = kBlock * kRowBytes;     // one of K, V
   static constexpr int kRing = NW * S * 2 * kTile;
-  static constexpr int kHeads = 8 * NT;
   // warps' states at a merge: m and sum, then O
   static int merge_bytes(int heads) { return NW * heads * (8 + D * 4); }
   static int bytes(int heads, int rows) { return kRing + merge_bytes(heads) + NW * S * 4 + rows * 8; }
 };
 
-template <class T, int NW, int D, int NT, int S>
+// CLUSTER: one cluster of CTAs per (request, pass) instead of equal ranges: the CTAs share its
+// blocks evenly and join through distributed shared memory.  One launch, no workspace.
+template <class T, int NW, int D, int NT, int S, bool CLUSTER>
 __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_constant__ DecodeArgs a) {
   using Shape = DecodeShape<NW, D, NT, S>;
   constexpr int kThreads = NW * 32;
@@ -124,11 +151,12 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   constexpr float kShift = std::is_same<T, OpF16>::value ? 7.f : 0.f;
   extern __shared__ __align__(128) char smem[];
   __shared__ int64_t s_warp_total[NW];
+  __shared__ int s_warp_live[NW];
   __shared__ Segment s_start;
+  __shared__ float2 s_cta[8 * NT];
 
   // the joining launch may begin to set itself up; it waits for this grid before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int heads = a.heads_per_pass;
   char *ring = smem;
@@ -138,79 +166,128 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   int *s_first = s_mask + NW * S;                                          // [rows]
   int *s_len = s_first + a.rows;                                           // [rows]
 
-  // ---- the batch: lengths, this CTA's range, where in the batch it begins
+  // ---- what this CTA works on: blocks of one (request, pass), or a range of the whole batch's
   const int passes = a.c.kv_heads * a.head_blocks;
-  const int per = (a.rows + kThreads - 1) / kThreads;
   const auto blocks_of = [&](int len) {
     const int lo = a.window > 0 && len > a.window ? len - a.window : 0;
     return (len + kBlock - 1) / kBlock - lo / kBlock;
   };
-  int64_t mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int r = tid * per + i;
-    if (r >= a.rows) break;
-    const PagedRun run = paged_run(a.c.indptr[r], a.c.indptr[r + 1], a.c.last[r], a.c.page_size, a.c.num_indices);
-    if (run.broken && blockIdx.x == 0) paged_flag(a.c, kPagedBadTable);
-    s_first[r] = int(run.first);
-    s_len[r] = int(run.tokens);
-    mine += int64_t(blocks_of(int(run.tokens))) * passes;
-  }
-  int64_t before = mine;            // inclusive scan over the threads
-#pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const int64_t x = __shfl_up_sync(~0u, before, o);
-    if (lane >= o) before += x;
-  }
-  if (lane == 31) s_warp_total[warp] = before;
-  __syncthreads();
-  int64_t total = 0;
-  before -= mine;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if (w < warp) before += s_warp_total[w];
-    total += s_warp_total[w];
-  }
-  const int64_t want = total / kMinUnits;
-  const int workers = want < 1 ? 1 : want < int64_t(gridDim.x) ? int(want) : int(gridDim.x);
-  const bool works = total > 0 && int(blockIdx.x) < workers;
-  const int64_t u0 = works ? range_start(total, blockIdx.x, workers) : 0;
-  const int64_t u1 = works ? range_start(total, blockIdx.x + 1, workers) : 0;
+  int one_first = 0, one_len = 0;       // CLUSTER: of its request
   const auto fill = [&](Segment &s) {   // what follows from the request
-    s.first = s_first[s.r];
-    s.len = s_len[s.r];
+    s.first = CLUSTER ? one_first : s_first[s.r];
+    s.len = CLUSTER ? one_len : s_len[s.r];
     s.lo = a.window > 0 && s.len > a.window ? s.len - a.window : 0;
     s.b0 = s.lo / kBlock;
     s.nb = blocks_of(s.len);
   };
-  if (works && u0 >= before && u0 < before + mine) {
-    int64_t off = u0 - before;
-    Segment s;
-    for (s.r = tid * per;; ++s.r) {
-      fill(s);
-      if (off < int64_t(s.nb) * passes) break;
-      off -= int64_t(s.nb) * passes;
+  // Both ends of a range inside a short segment move to an end of it, the same way for the two
+  // ranges that meet there.
+  const auto snap = [&](Segment &s) {
+    if (s.nb > kSnapUnits) return;
+    s.jb = s.jb == s.nb || 2 * s.jb > s.nb ? s.nb : 0;
+    s.ja = s.ja == 0 || 2 * s.ja <= s.nb ? 0 : s.nb;
+    if (s.ja >= s.jb) s.ja = s.jb = 0;
+  };
+  Segment begin;
+  Ranges all = {};
+  int64_t u1 = 0;
+  const int ctas = CLUSTER ? a.ctas : 1, rank = CLUSTER ? int(blockIdx.x) % ctas : 0;
+  if (CLUSTER) {
+    const int seg = int(blockIdx.x) / ctas;
+    begin.r = seg / passes;
+    begin.pass = seg % passes;
+    const PagedRun run = paged_run(a.c.indptr[begin.r], a.c.indptr[begin.r + 1], a.c.last[begin.r], a.c.page_size,
+                                   a.c.num_indices);
+    if (run.broken && tid == 0) paged_flag(a.c, kPagedBadTable);
+    one_first = int(run.first);
+    one_len = int(run.tokens);
+    fill(begin);
+    begin.ja = int(int64_t(begin.nb) * rank / ctas);
+    begin.jb = int(int64_t(begin.nb) * (rank + 1) / ctas);
+    begin.left = 0;
+  } else {
+    const int per = (a.rows + kThreads - 1) / kThreads;
+    int64_t mine = 0;
+    int requests = 0;             // that have positions
+    for (int i = 0; i < per; ++i) {
+      const int r = tid * per + i;
+      if (r >= a.rows) break;
+      const PagedRun run = paged_run(a.c.indptr[r], a.c.indptr[r + 1], a.c.last[r], a.c.page_size, a.c.num_indices);
+      if (run.broken && blockIdx.x == 0) paged_flag(a.c, kPagedBadTable);
+      s_first[r] = int(run.first);
+      s_len[r] = int(run.tokens);
+      mine += int64_t(blocks_of(int(run.tokens))) * passes;
+      requests += run.tokens > 0;
     }
-    s.pass = int(off / s.nb);
-    s.ja = int(off % s.nb);
-    s.jb = int(min(int64_t(s.nb), s.ja + (u1 - u0)));
-    s.left = (u1 - u0) - (s.jb - s.ja);
-    s_start = s;
-  }
-  if (tid == 0) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
-  // requests without positions: nobody's range
-  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    // (s_len of r was written by this CTA before the barrier above)
-    if (s_len[r] != 0) continue;
-    for (int i = tid; i < a.q_heads * (D / 8); i += kThreads) {
-      const int h = i / (D / 8);
-      *reinterpret_cast<uint4 *>(a.out + 2 * (r * a.o_token + (h / a.group) * a.o_group + (h % a.group) * a.o_head) +
-                                 16 * (i % (D / 8))) = make_uint4(0, 0, 0, 0);
+    int64_t before = mine;            // inclusive scan over the threads
+  #pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int64_t x = __shfl_up_sync(~0u, before, o);
+      if (lane >= o) before += x;
     }
-    if (a.lse)
-      for (int h = tid; h < a.q_heads; h += kThreads) a.lse[int64_t(r) * a.q_heads + h] = -INFINITY;
+    requests = __reduce_add_sync(~0u, requests);
+    if (lane == 31) {
+      s_warp_total[warp] = before;
+      s_warp_live[warp] = requests;
+    }
+    __syncthreads();
+    int64_t total = 0;
+    requests = 0;
+    before -= mine;
+  #pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) before += s_warp_total[w];
+      total += s_warp_total[w];
+      requests += s_warp_live[w];
+    }
+    all.total = total;
+    // As many workers as have kMinUnits each, or as there are segments; and where a worker's share
+    // is short, a whole number per segment, so that equal segments are cut at their ends (a
+    // second segment in a range costs about as much as kAlignUnits).
+    const int segments = requests * passes;
+    int workers = int(max(int64_t(1), min(max(total / kMinUnits, int64_t(segments)), int64_t(gridDim.x))));
+    if (segments > 0 && segments <= workers && total < int64_t(kAlignUnits) * workers)
+      workers -= workers % segments;
+    all.workers = workers;
+    all.each = divide(total, all.workers);
+    all.more = int(total - all.each * all.workers);
+    const bool works = total > 0 && int(blockIdx.x) < all.workers;
+    const int64_t u0 = all.start(blockIdx.x);
+    u1 = all.start(blockIdx.x + 1);
+    if (works && u0 >= before && u0 < before + mine) {
+      int64_t off = u0 - before;
+      Segment s;
+      for (s.r = tid * per;; ++s.r) {
+        fill(s);
+        if (off < int64_t(s.nb) * passes) break;
+        off -= int64_t(s.nb) * passes;
+      }
+      s.pass = int(divide(off, s.nb));
+      s.ja = int(off - int64_t(s.pass) * s.nb);
+      s.jb = int(min(int64_t(s.nb), s.ja + (u1 - u0)));
+      s.left = (u1 - u0) - (s.jb - s.ja);
+      snap(s);
+      s_start = s;
+    }
+    if (tid == 0 && !a.by_segment) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
+    // requests without positions: nobody's range
+    for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+      // (s_len of r was written by this CTA before the barrier above)
+      if (s_len[r] != 0) continue;
+      if (a.by_segment)
+        for (int i = tid; i < passes; i += kThreads) a.desc[r * passes + i] = make_int4(0, 0, 0, 0);
+      for (int i = tid; i < a.q_heads * (D / 8); i += kThreads) {
+        const int h = i / (D / 8);
+        *reinterpret_cast<uint4 *>(a.out + 2 * (r * a.o_token + (h / a.group) * a.o_group + (h % a.group) * a.o_head) +
+                                   16 * (i % (D / 8))) = make_uint4(0, 0, 0, 0);
+      }
+      if (a.lse)
+        for (int h = tid; h < a.q_heads; h += kThreads) a.lse[int64_t(r) * a.q_heads + h] = -INFINITY;
+    }
+    __syncthreads();
+    if (!works) return;
+    begin = s_start;
   }
-  __syncthreads();
-  if (!works) return;
 
   const auto next_segment = [&](Segment &s) {   // only while s.left > 0
     if (++s.pass == passes) {
@@ -222,12 +299,13 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     s.ja = 0;
     s.jb = int(min(int64_t(s.nb), s.left));
     s.left -= s.jb;
+    snap(s);
   };
 
   // ---- filling the ring: this warp's blocks one after the other, across segments
   char *my_ring = ring + warp * (S * 2 * Shape::kTile);
   const uint32_t my_ring32 = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
-  Segment fs = s_start;
+  Segment fs = begin;
   int fj = fs.ja + warp;
   int page = 0;                // of this lane's row (lane % 16) in the block at the cursor
   bool more = true;            // the cursor stands on a block
@@ -276,21 +354,34 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
 
   // ---- consuming
   int stage = 0;
-  Segment cs = s_start;
-  for (;;) {
-    const int kv = cs.pass / a.head_blocks, h0 = (cs.pass % a.head_blocks) * heads;
-    const int live = min(heads, a.group - h0);        // query heads of this pass
-    uint32_t qf[NT][D / 16][2];
+  Segment cs = begin;
+  uint32_t qf[NT][D / 16][2];       // of the segment in work
+  const auto load_q = [&](const Segment &s) {
+    const int kv = s.pass / a.head_blocks, h0 = (s.pass % a.head_blocks) * heads;
+    const int live = min(heads, a.group - h0);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int h = n * 8 + lane / 4;
-      const char *qp = a.q + 2 * (cs.r * a.q_token + kv * a.q_group + (h0 + h) * a.q_head) + (lane % 4) * 4;
+      const char *qp = a.q + 2 * (s.r * a.q_token + kv * a.q_group + (h0 + h) * a.q_head) + (lane % 4) * 4;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        qf[n][ks][0] = h < live ? *reinterpret_cast<const uint32_t *>(qp + ks * 32) : 0u;
-        qf[n][ks][1] = h < live ? *reinterpret_cast<const uint32_t *>(qp + ks * 32 + 16) : 0u;
+        qf[n][ks][0] = h < live ? __ldg(reinterpret_cast<const uint32_t *>(qp + ks * 32)) : 0u;
+        qf[n][ks][1] = h < live ? __ldg(reinterpret_cast<const uint32_t *>(qp + ks * 32 + 16)) : 0u;
       }
     }
+  };
+  const auto advance = [&]() {      // to the next segment that has blocks in this range
+    do {
+      if (cs.left == 0) return false;
+      next_segment(cs);
+    } while (cs.ja >= cs.jb);
+    return true;
+  };
+  if (!CLUSTER && cs.ja >= cs.jb && !advance()) return;
+  for (;;) {
+    load_q(cs);
+    const int kv = cs.pass / a.head_blocks, h0 = (cs.pass % a.head_blocks) * heads;
+    const int live = min(heads, a.group - h0);        // query heads of this pass
     float o[NT][D / 16][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -399,14 +490,11 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
         }
       }
     __syncthreads();
-    const bool whole = cs.ja == 0 && cs.jb == cs.nb;
-    const int slot = 2 * blockIdx.x + (cs.ja == 0);    // 1: the range that begins the segment
-    for (int i = tid; i < live * (D / 4); i += kThreads) {
-      const int h = i / (D / 4), d = i % (D / 4) * 4;
-      float top = -INFINITY, sum = 0.f;
+    const auto warps_joined = [&](int h, int d, float &top, float &sum, float4 &x) {
+      top = -INFINITY, sum = 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) top = fmaxf(top, m_ml[w * heads + h].x);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const float2 ml = m_ml[w * heads + h];
@@ -415,75 +503,137 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
         sum += f * ml.y;
         x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
       }
+    };
+    const auto finish = [&](int h, int d, float top, float sum, const float4 &x) {
+      const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+      const uint2 v = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
+      *reinterpret_cast<uint2 *>(a.out + 2 * (cs.r * a.o_token + kv * a.o_group + (h0 + h) * a.o_head + d)) = v;
+      if (a.lse && d == 0)
+        a.lse[int64_t(cs.r) * a.q_heads + kv * a.group + h0 + h] =
+            sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.69314718055994531f;
+    };
+    if (CLUSTER) {
+      cg::cluster_group cluster = cg::this_cluster();
+      // this CTA's state where the first warp's was, then the cluster's CTAs share the output
+      for (int i = tid; i < live * (D / 4); i += kThreads) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float top, sum;
+        float4 x;
+        warps_joined(h, d, top, sum, x);
+        *reinterpret_cast<float4 *>(m_o + h * D + d) = x;
+        if (d == 0) s_cta[h] = make_float2(top, sum);
+      }
+      cluster.sync();
+      for (int i = tid * ctas + rank; i < live * (D / 4); i += kThreads * ctas) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -INFINITY, sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float2 ml[kMaxCluster];
+        float4 y[kMaxCluster];
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) {
+          if (c >= ctas) break;
+          ml[c] = cluster.map_shared_rank(s_cta, c)[h];
+          y[c] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(m_o, c) + h * D + d);
+          top = fmaxf(top, ml[c].x);
+        }
+#pragma unroll
+        for (int c = 0; c < kMaxCluster; ++c) {
+          if (c >= ctas) break;
+          const float f = ml[c].y == 0.f ? 0.f : exp2_fast(ml[c].x - top);
+          sum += f * ml[c].y;
+          x.x += f * y[c].x, x.y += f * y[c].y, x.z += f * y[c].z, x.w += f * y[c].w;
+        }
+        finish(h, d, top, sum, x);
+      }
+      cluster.sync();     // nobody leaves while its shared memory is read
+      return;
+    }
+    const bool whole = cs.ja == 0 && cs.jb == cs.nb;
+    const int slot = 2 * blockIdx.x + (cs.ja == 0);    // 1: the range that begins the segment
+    for (int i = tid; i < live * (D / 4); i += kThreads) {
+      const int h = i / (D / 4), d = i % (D / 4) * 4;
+      float top, sum;
+      float4 x;
+      warps_joined(h, d, top, sum, x);
       if (whole) {
-        const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
-        const uint2 v = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
-        *reinterpret_cast<uint2 *>(a.out + 2 * (cs.r * a.o_token + kv * a.o_group + (h0 + h) * a.o_head + d)) = v;
-        if (a.lse && d == 0)
-          a.lse[int64_t(cs.r) * a.q_heads + kv * a.group + h0 + h] =
-              sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.69314718055994531f;
+        finish(h, d, top, sum, x);
       } else {
         *reinterpret_cast<float4 *>(a.part_o + (int64_t(slot) * heads + h) * D + d) = x;
         if (d == 0) a.part_ml[int64_t(slot) * heads + h] = make_float2(top, sum);
       }
     }
-    if (!whole && cs.ja == 0 && tid == 0) {
-      // this range begins the segment: tell the joining launch how many ranges it runs through
-      const int64_t end = u1 + (cs.nb - cs.jb);       // one past the segment's last unit
-      int last = int(min(int64_t(workers - 1), (end - 1) * workers / total));
-      while (last + 1 < workers && range_start(total, last + 1, workers) <= end - 1) ++last;
-      while (range_start(total, last, workers) > end - 1) --last;
-      a.desc[blockIdx.x] = make_int4(cs.r, cs.pass, last - int(blockIdx.x) + 1, 0);
+    if (cs.ja == 0 && tid == 0 && (!whole || a.by_segment)) {
+      // this range begins the segment: how many does it run through?
+      const int parts = whole ? 0 : all.owner(u1 + (cs.nb - cs.jb) - 1) - int(blockIdx.x) + 1;
+      a.desc[a.by_segment ? cs.r * passes + cs.pass : int(blockIdx.x)] = make_int4(cs.r, cs.pass, parts, blockIdx.x);
     }
-    if (cs.left == 0) break;
+    if (!advance()) break;
     __syncthreads();      // the merge area is free again
-    next_segment(cs);
   }
 }
 
-// Joins the parts of the segment that begins in worker blockIdx.x's range, for query head
-// blockIdx.y of the pass: parts of workers x (slot 1), x + 1, ... (slot 0).
+// Joins the parts of one segment (blockIdx.x: see DecodeArgs::by_segment) for query head
+// blockIdx.y of the pass and D / gridDim.z dimensions: parts of workers c (slot 1), c + 1, ...
+// (slot 0).  One pass, each group of threads over its own parts, kAhead rows of them in flight.
 template <class T, int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ DecodeArgs a) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes;      // threads per row, rows at a time
+  constexpr int kAhead = 8;
   constexpr float kShift = std::is_same<T, OpF16>::value ? 7.f : 0.f;
-  __shared__ float s_red[8];
-  __shared__ float s_sum[kGroups];
-  __shared__ float4 s_o[kGroups][kLanes];
+  __shared__ float2 s_ml[32];
+  __shared__ float4 s_o[256];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 desc = a.desc[blockIdx.x];
   const int parts = desc.z, heads = a.heads_per_pass, h = blockIdx.y;
   const int kv = desc.y / a.head_blocks, h0 = (desc.y % a.head_blocks) * heads;
   if (parts == 0 || h0 + h >= a.group) return;
-  const auto row_of = [&](int i) { return (int64_t(2) * (blockIdx.x + i) + (i == 0)) * heads + h; };
-  float top = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += 256) top = fmaxf(top, a.part_ml[row_of(i)].x);
-#pragma unroll
-  for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-  if (threadIdx.x % 32 == 0) s_red[threadIdx.x / 32] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) top = fmaxf(top, s_red[w]);
-  const int g = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
+  const int lanes = gridDim.z > 1 ? 8 : D / 4;               // threads per row
+  const int groups = 256 / lanes;                            // rows at a time
+  const int g = threadIdx.x / lanes, d = blockIdx.z * 8 + threadIdx.x % lanes;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-#pragma unroll 8
-  for (int i = g; i < parts; i += kGroups) {
-    const float2 ml = a.part_ml[row_of(i)];
-    const float4 y = *reinterpret_cast<const float4 *>(a.part_o + row_of(i) * D + d * 4);
-    const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);
-    sum += f * ml.y;
-    x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
+  float top = -INFINITY, sum = 0.f;
+  for (int i0 = g; i0 < parts; i0 += groups * kAhead) {
+    float2 ml[kAhead];
+    float4 y[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int i = i0 + j * groups;
+      ml[j] = make_float2(-INFINITY, 0.f);
+      y[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i < parts) {
+        const int64_t row = (int64_t(2) * (desc.w + i) + (i == 0)) * heads + h;
+        ml[j] = a.part_ml[row];
+        y[j] = *reinterpret_cast<const float4 *>(a.part_o + row * D + d * 4);
+      }
+    }
+    float next = top;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) next = fmaxf(next, ml[j].x);
+    const float keep = sum == 0.f ? 0.f : exp2_fast(top - next);
+    sum = sum == 0.f ? 0.f : sum * keep;
+    x.x *= keep, x.y *= keep, x.z *= keep, x.w *= keep;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float f = ml[j].y == 0.f ? 0.f : exp2_fast(ml[j].x - next);   // (a NaN sum stays one)
+      sum += f * ml[j].y;
+      x.x += f * y[j].x, x.y += f * y[j].y, x.z += f * y[j].z, x.w += f * y[j].w;
+    }
+    top = next;
   }
-  s_o[g][d] = x;
-  if (d == 0) s_sum[g] = sum;
+  s_o[threadIdx.x] = x;
+  if (threadIdx.x % lanes == 0) s_ml[g] = make_float2(top, sum);
   __syncthreads();
   if (g != 0) return;
-#pragma unroll
-  for (int i = 1; i < kGroups; ++i) {
-    const float4 y = s_o[i][d];
-    sum += s_sum[i];
-    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+  const int used = min(groups, parts);
+  for (int i = 1; i < used; ++i) top = fmaxf(top, s_ml[i].x);
+  sum = 0.f;
+  x = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < used; ++i) {
+    const float2 ml = s_ml[i];
+    const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);
+    const float4 y = s_o[i * lanes + threadIdx.x];
+    sum += f * ml.y;
+    x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
   }
   const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
   const uint2 v = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
@@ -524,29 +674,46 @@ uint64_t workspace_bytes(int workers, int heads, int head_dim) {
 
 constexpr int kMaxShared = 232448 - 1024;   // opt-in limit of a block, less the static part
 
-template <class T, int NW, int D, int NT, int S>
+template <class T, int NW, int D, int NT, int S, bool CLUSTER>
 int launch_shape(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
   using Shape = DecodeShape<NW, D, NT, S>;
   static std::atomic<uint64_t> ready{0};      // devices whose limit has been raised
-  auto *kernel = paged_decode_kernel<T, NW, D, NT, S>;
+  auto *kernel = paged_decode_kernel<T, NW, D, NT, S, CLUSTER>;
+  cudaError_t e = cudaSuccess;
   if (!(ready.load(std::memory_order_relaxed) >> dev.device & 1)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
     if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: shared memory: %s", cudaGetErrorString(e));
     ready.fetch_or(uint64_t(1) << dev.device, std::memory_order_relaxed);
   }
-  kernel<<<dev.sms, NW * 32, Shape::bytes(a.heads_per_pass, a.rows), st>>>(a);
-  if (int rc = op_launched("paged_decode")) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(dev.sms, a.heads_per_pass);
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(dev.sms);
+  cfg.blockDim = dim3(NW * 32);
+  cfg.dynamicSmemBytes = Shape::bytes(a.heads_per_pass, CLUSTER ? 0 : a.rows);
+  cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a);
-  if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: joining launch: %s", cudaGetErrorString(e));
+  cfg.numAttrs = 0;
+  if (CLUSTER) {
+    cfg.gridDim = dim3(unsigned(a.rows) * a.c.kv_heads * a.head_blocks * a.ctas);
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e == cudaSuccess && !CLUSTER) {
+    // few segments: many threads on each (32 dimensions a block)
+    const int segments = a.rows * a.c.kv_heads * a.head_blocks;
+    const bool fine = a.by_segment && segments * a.heads_per_pass * (D / 32) <= 4 * dev.sms;
+    cfg.gridDim = dim3(a.by_segment ? segments : dev.sms, a.heads_per_pass, fine ? D / 32 : 1);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a);
+  }
+  if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: launch: %s", cudaGetErrorString(e));
   return YPK_OK;
 }
 
@@ -554,9 +721,25 @@ int launch_shape(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
 // thousands of requests need the room.
 template <class T, int NW, int D, int NT>
 int launch_ring(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
-  if (DecodeShape<NW, D, NT, 3>::bytes(a.heads_per_pass, a.rows) <= kMaxShared)
-    return launch_shape<T, NW, D, NT, 3>(a, dev, st);
-  return launch_shape<T, NW, D, NT, 2>(a, dev, st);
+  constexpr int kDeep = NT == 2 && D == 128 ? 2 : 3;
+  if (a.ctas) return launch_shape<T, NW, D, NT, kDeep, true>(a, dev, st);
+  if (kDeep == 3 && DecodeShape<NW, D, NT, 3>::bytes(a.heads_per_pass, a.rows) <= kMaxShared)
+    return launch_shape<T, NW, D, NT, kDeep, false>(a, dev, st);
+  return launch_shape<T, NW, D, NT, 2, false>(a, dev, st);
+}
+
+// CTAs per (request, pass) when each gets a cluster of its own, 0: equal ranges.  A cluster is
+// one launch and joins inside it, but a long request among short ones is its cluster's alone.
+// How long it can be is known on the host only as far as the page list goes: clusters are used
+// where even the whole list in one request's hands leaves a CTA at most kClusterUnits.
+constexpr int kClusterUnits = 64;
+int cluster_ctas(const ypk_paged_cache *c, int rows, int passes, int window, int sms) {
+  int64_t units = (int64_t(c->num_indices) * c->page_size + kBlock - 1) / kBlock;
+  if (window > 0) units = std::min(units, int64_t(window) / kBlock + 2);
+  const int64_t segments = int64_t(rows) * passes;
+  int ctas = 1;
+  while (ctas < kMaxCluster && segments * ctas * 2 <= sms && units > 8 * ctas) ctas *= 2;
+  return units <= int64_t(kClusterUnits) * ctas && segments * ctas < 0x7fffffff ? ctas : 0;
 }
 
 template <class T>
@@ -618,6 +801,8 @@ extern "C" int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_de
   a.window = p->window;
   a.heads_per_pass = pass_heads(cache->head_dim, a.group);
   a.head_blocks = (a.group + a.heads_per_pass - 1) / a.heads_per_pass;
+  a.ctas = cluster_ctas(cache, p->rows, cache->num_kv_heads * a.head_blocks, p->window, dev.sms);
+  a.by_segment = int64_t(p->rows) * cache->num_kv_heads * a.head_blocks <= dev.sms;
   a.scale_log2 = p->scale * 1.4426950408889634f;
   const uint64_t need = workspace_bytes(dev.sms, a.heads_per_pass, cache->head_dim);
   if (!p->workspace || p->workspace_bytes < need)
