@@ -572,9 +572,42 @@ def test_logprobs_masked_rows(dtype):
     x[7] = torch.finfo(dtype).max
     x[8, :5] = torch.finfo(dtype).max
     got = check_logprobs(x, torch.tensor([0, 0, 3999, 7, 4, 3, 15, 9, 2], device="cuda"), 12)
-    assert got.entropy[0] == 0 and got.entropy[1] == 0 and (got.top_logprob[0] == ninf).all()
+    # one column: ln 2 (log2 2^e - e), e the rounding of the reference, both functions within 2 ulp
+    # of a number next to 1: 2^-21
+    assert got.entropy[0] == 0 and 0 <= got.entropy[1] <= 2 ** -21 and (got.top_logprob[0] == ninf).all()
     assert got.top_token[0].tolist() == list(range(12))
     assert abs(got.entropy[4].item() - math.log(4000)) < 1e-3
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [1, 150])
+def test_logprobs_far_values(dtype, rows):
+    """Rows at every distance from zero: values and masks around the borders of the exponent's range.
+    A weight is then off by 2^-24 of the reference's size more, as y = x log2 e - r is: far rows
+    get that on top of the bound, which check_logprobs takes for values of ordinary size."""
+    g = gen(40)
+    big = torch.finfo(dtype).max
+    for base in (0.0, 100.0, 6e4, 1e6, 1e9, 2.0 ** 30, 2.0 ** 31, 1e10, 1e30, 2.3e38, 3.3e38):
+        for sign in (1, -1):
+            if base > big:
+                continue
+            x = (torch.randn(rows, 9000, generator=g, device="cuda") + sign * base).clamp(-big, big).to(dtype)
+            x[:, 7000:] = -big
+            x[:, 8000:] = float("-inf")
+            t = torch.randint(0, 9000, (rows,), generator=g, device="cuda")
+            got = yr.token_logprobs(x, t, top_k=3)
+            want = torch.log_softmax(x.to(F64), 1)
+            p = want.exp()
+            entropy = -torch.where(p > 0, p * want, 0.0).sum(1)
+            off = 2 ** -14 * (1 + entropy) + 2 ** -22 * min(base, 2.0 ** 30) * 2 ** -7
+            assert ((got.entropy.to(F64) - entropy).abs() <= off).all(), (base, sign)
+            lp, w = got.logprob.to(F64), want.gather(1, t[:, None])[:, 0]
+            w = torch.where(torch.isinf(w.to(F32)), float("-inf"), w)        # more than fp32 holds
+            seen = w > float("-inf")
+            assert torch.equal(lp > float("-inf"), seen)
+            assert ((lp - w).abs()[seen] <= (2 ** -15 + 2 ** -22 * min(base, 2.0 ** 30) * 2 ** -7 + 2 ** -22 * w.abs())[seen]).all()
+            at = torch.topk(order_keys(x) * (1 << 20) - torch.arange(9000, device="cuda"), 3, 1).indices
+            assert torch.equal(got.top_token, at)
 
 
 @pytest.mark.parametrize("rows", [1, 200])

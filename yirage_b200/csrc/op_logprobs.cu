@@ -1,22 +1,26 @@
 // Log probabilities of given tokens, with entropy and top alternatives (ypk_token_logprobs).
 //
-//   m = max x,  s = sum e^(x - m),  u = sum (x - m) e^(x - m)
-//   log p(t) = x_t - m - ln s,   entropy = ln s - u / s
+//   y = x log2 e - r,  s = sum 2^y,  u = sum y 2^y      (r: the running maximum's x log2 e)
+//   log2 p(t) = y_t - log2 s,   entropy = ln 2 (log2 s - u / s)
 //
-// One pass over the logits with m, s and u running in each thread's registers (in the base 2:
-// y = (x - m) log2 e).  Memory bounds it; next comes the exponential, one per logit: 73 % of the
-// special-function rate when 16-bit logits arrive at the copy rate, so everything else is kept
-// to packed pairs (two fp32 per instruction, maxima on pairs of 16-bit values).
+// One pass over the logits with r, s and u running in each thread's registers.  r is rounded, but
+// the same rounded number stands in every y, so it cancels.  Memory bounds the pass only if it
+// stays under about seven instructions a logit at 16 bits (four schedulers, 6.5 TB/s), and the
+// exponential alone takes 73 % of its unit at that rate: so pairs of fp32 share an instruction
+// (fma.f32x2), maxima and the clamp are taken on pairs of 16-bit values.  The clamp keeps
+// -infinity out of the products: a column so low adds nothing while the maximum is above kLow; a
+// row whose maximum is not, or is above kHigh, has only weights of 0 and 1, and its maxima are
+// counted instead.
 //
-// The top alternatives cost the pass nothing.  Its running maxima m_t, one per thread, give a
-// bound: the k-th largest maximum of 64 groups of threads is at most the k-th largest logit.
-// Only the columns of the threads whose own maximum reaches the bound (about k of 512) are read
-// again, from L2, and what reaches the bound there (a little more than k logits) is ranked.
-// Rows full of equal values (a mask that leaves less than k columns) overflow that list; they
-// take the logits above the bound and then the lowest columns that equal it.
+// The top alternatives cost the pass nothing.  Its running maxima, one per thread, give a bound:
+// the k-th largest maximum of 64 groups of threads is at most the k-th largest logit.  Only the
+// columns of the threads whose own maximum reaches the bound (little more than k) are read
+// again, from L2, and what reaches the bound there is ranked.  Rows full of equal values (a mask
+// that leaves less than k columns) overflow that list; they take the slow way: the logits above
+// the bound and then the lowest columns that equal it.
 //
-// A row is split over a cluster of CTAs when there are few rows; their sums and lists are
-// joined through distributed shared memory, so there is no workspace and no second launch.
+// A row is split over a cluster of CTAs when there are few rows; bounds, sums and candidates
+// travel through distributed shared memory, so there is no workspace and no second launch.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -31,15 +35,20 @@ namespace ypk {
 namespace {
 
 constexpr int kMaxTop = 32;
-constexpr int kThreads = 512;
-constexpr int kGroups = 64;        // of 8 threads: what the bound of the top list is taken from
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kGroups = 64;        // of 4 threads: what the bound of a slice's top list is taken from
+constexpr int kMaxGroups = 128;    // over a cluster
 constexpr int kCandidates = 1024;
 constexpr int kUnroll = 4;         // 16-byte loads in flight per thread (and as many ahead)
 constexpr int kMaxCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
-// Exponents below this add nothing to a sum that holds a 1; it keeps -infinity out of products.
+// Exponents below this add nothing to a sum that holds a 1.
 constexpr float kFloor = -200.f;
+// Beyond kHigh (and below Vec::kLow) neighbouring values are at least 32 apart: weights are 0 or 1.
+// Up to there the rounding of the reference shifts every y by at most 2^-24 of it, under 100.
+constexpr float kHigh = 0x1p30f;
 
 struct LogprobArgs {
   const char *logits;
@@ -115,6 +124,13 @@ struct Vec;
 template <>
 struct Vec<YPK_F32> {
   static constexpr int kN = 4, kBytes = 4;
+  static constexpr float kLow = -0x1p30f;
+  static __device__ __forceinline__ uint32_t clamp1(uint32_t v) {
+    return __float_as_uint(fmaxf(__uint_as_float(v), -0x1p34f));
+  }
+  static __device__ __forceinline__ uint4 clamp(const uint4 &v) {
+    return make_uint4(clamp1(v.x), clamp1(v.y), clamp1(v.z), clamp1(v.w));
+  }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
   static __device__ __forceinline__ float top(const uint4 &v) {
     return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
@@ -127,6 +143,15 @@ struct Vec<YPK_F32> {
 template <>
 struct Vec<YPK_BF16> {
   static constexpr int kN = 8, kBytes = 2;
+  static constexpr float kLow = -0x1p30f;
+  static __device__ __forceinline__ uint32_t clamp2(uint32_t v) {      // to -2^34
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0xd080d080u));
+    return r;
+  }
+  static __device__ __forceinline__ uint4 clamp(const uint4 &v) {
+    return make_uint4(clamp2(v.x), clamp2(v.y), clamp2(v.z), clamp2(v.w));
+  }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -147,6 +172,15 @@ struct Vec<YPK_BF16> {
 template <>
 struct Vec<YPK_F16> {
   static constexpr int kN = 8, kBytes = 2;
+  static constexpr float kLow = -60000.f;
+  static __device__ __forceinline__ uint32_t clamp2(uint32_t v) {      // to the lowest value, -65504
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0xfbfffbffu));
+    return r;
+  }
+  static __device__ __forceinline__ uint4 clamp(const uint4 &v) {
+    return make_uint4(clamp2(v.x), clamp2(v.y), clamp2(v.z), clamp2(v.w));
+  }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
   static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -165,40 +199,45 @@ struct Vec<YPK_F16> {
   }
 };
 
-// Running maximum and sums.
+// Sums against a reference, and the true maximum (NaN if there is one).
 struct Sums {
-  float m, s, u;
+  float r, s, u, top;
 };
+constexpr Sums kNoSums = {-INFINITY, 0.f, 0.f, -INFINITY};
 
-// To the reference `top` (>= m, or NaN).
-__device__ __forceinline__ void move_reference(Sums &a, float top) {
-  const float d = fmaxf((a.m - top) * kLog2e, kFloor);   // (-infinity and NaN: no weight is lost, s = 0)
-  const float f = exp2_fast(d);
-  a.u = a.s == 0.f ? 0.f : (a.u + d * a.s) * f;
-  a.s = a.s == 0.f ? 0.f : a.s * f;
-  a.m = top;
+__device__ __forceinline__ void join(Sums &a, const Sums &b) {
+  const float r = fmaxf(a.r, b.r);
+  const float da = fmaxf(a.r - r, kFloor), db = fmaxf(b.r - r, kFloor);   // (none yet: NaN or -infinity, s = 0)
+  const float fa = exp2_fast(da), fb = exp2_fast(db);
+  a.u = (a.u + da * a.s) * fa + (b.u + db * b.s) * fb;
+  a.s = a.s * fa + b.s * fb;
+  a.r = r;
+  a.top = max_nan(a.top, b.top);
 }
 
-__device__ __forceinline__ void join(Sums &a, Sums b) {
-  const float top = max_nan(a.m, b.m);
-  move_reference(a, top);
-  move_reference(b, top);
-  a.s += b.s;
-  a.u += b.u;
+__device__ __forceinline__ Sums shuffled(const Sums &a, int x) {
+  Sums o;
+  o.r = __shfl_xor_sync(~0u, a.r, x);
+  o.s = __shfl_xor_sync(~0u, a.s, x);
+  o.u = __shfl_xor_sync(~0u, a.u, x);
+  o.top = __shfl_xor_sync(~0u, a.top, x);
+  return o;
 }
 
 struct Shared {
-  Sums warp[kThreads / 32];
-  Sums all;                               // of this CTA
-  uint32_t group[kGroups];
+  Sums warp[kWarps];
+  Sums row;                               // of the whole row
+  uint32_t part[kGroups];                 // maxima of this CTA's groups of threads
+  uint32_t group[kMaxGroups];             // of the row's
   uint32_t bound;
+  int slow;                               // the row has a NaN, or too many candidates
   int listed, found;
   int threads[kThreads];                  // whose columns are read again
   unsigned long long cand[kCandidates];
-  unsigned long long top[kMaxTop];        // of this CTA, falling; 0: none
+  unsigned long long top[kMaxTop];        // falling; 0: none
   unsigned long long best;
   unsigned long long merged[kMaxCluster * kMaxTop];
-  int warp_count[kThreads / 32];
+  int warp_count[kWarps];
 };
 
 // The columns of one CTA: a few single ones, whole 16-byte vectors, a few single ones.
@@ -224,27 +263,61 @@ __device__ __forceinline__ Slice slice_of(const char *row, int vocab, int rank, 
   return s;
 }
 
-// The k largest of sh.cand[0..n) in order into sh.top; every thread calls.
-__device__ void rank_candidates(Shared &sh, int n, int k) {
+// The k largest of n keys in order into sh.top; every thread calls.
+__device__ void rank_keys(Shared &sh, const unsigned long long *keys, int n, int k) {
   for (int i = threadIdx.x; i < n; i += kThreads) {
-    const unsigned long long mine = sh.cand[i];
+    const unsigned long long mine = keys[i];
+    if (mine == 0) continue;
     int above = 0;
-    for (int j = 0; j < n; ++j) above += sh.cand[j] > mine;
+    for (int j = 0; j < n; ++j) above += keys[j] > mine;
     if (above < k) sh.top[above] = mine;
   }
 }
 
+// Puts the columns of this CTA's slice that are at least `least` in order into the list of `to`
+// (counted in to.found, as far as there is room), from the threads of sh.threads.
+template <int DTYPE>
+__device__ __forceinline__ void collect(Shared &sh, Shared &to, const Slice &s, int listed, uint32_t least) {
+  using V = Vec<DTYPE>;
+  const int tid = threadIdx.x, first_vec = s.first + s.head;
+  const char *vec0 = s.row + int64_t(first_vec) * V::kBytes;
+  const int rounds = (s.vecs + kThreads - 1) / kThreads;
+  const auto offer = [&](float x, int col) {
+    const uint32_t o = order_of(x);
+    if (o < least) return;
+    const int at = atomicAdd(&to.found, 1);
+    if (at < kCandidates) to.cand[at] = key_of(o, uint32_t(col));
+  };
+  for (int i = tid; i < listed * rounds; i += kThreads) {
+    const int v = i / listed * kThreads + sh.threads[i % listed];
+    if (v >= s.vecs) continue;
+    const uint4 x = load16(vec0 + int64_t(v) * 16);
+    if (order_of(V::top(x)) < least) continue;
+#pragma unroll
+    for (int e = 0; e < V::kN / 2; ++e) {
+      const float2 f = V::two(x, e);
+      offer(f.x, first_vec + v * V::kN + 2 * e);
+      offer(f.y, first_vec + v * V::kN + 2 * e + 1);
+    }
+  }
+  if (tid < s.head) offer(V::one(s.row + int64_t(s.first + tid) * V::kBytes), s.first + tid);
+  if (tid < s.tail) {
+    const int col = first_vec + s.vecs * V::kN + tid;
+    offer(V::one(s.row + int64_t(col) * V::kBytes), col);
+  }
+}
+
+// The slow way: the k largest of this CTA's slice, exactly, into sh.top.
 template <int DTYPE>
 __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
   using V = Vec<DTYPE>;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int first_vec = s.first + s.head;                      // column of the first vector
-  const char *vec0 = s.row + int64_t(first_vec) * V::kBytes;
   const int columns = s.head + s.vecs * V::kN + s.tail;
   const uint32_t mine = order_of(my_max);
   uint32_t g = mine;
 #pragma unroll
   for (int x = 1; x < kThreads / kGroups; x *= 2) g = max(g, __shfl_xor_sync(~0u, g, x));
+  __syncthreads();
   if (tid % (kThreads / kGroups) == 0) sh.group[tid / (kThreads / kGroups)] = g;
   if (tid < kMaxTop) sh.top[tid] = 0;
   if (tid == 0) sh.listed = sh.found = 0;
@@ -261,36 +334,8 @@ __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
     const uint32_t bound = sh.bound;
     if (mine >= bound) sh.threads[atomicAdd(&sh.listed, 1)] = tid;
     __syncthreads();
-    const int listed = sh.listed;
-    const int rounds = (s.vecs + kThreads - 1) / kThreads;
-    // logits of at least (strict: above) the bound, in no order
-    const auto collect = [&](uint32_t least) {
-      const auto offer = [&](float x, int col) {
-        const uint32_t o = order_of(x);
-        if (o < least) return;
-        const int at = atomicAdd(&sh.found, 1);
-        if (at < kCandidates) sh.cand[at] = key_of(o, uint32_t(col));
-      };
-      for (int i = tid; i < listed * rounds; i += kThreads) {
-        const int v = i / listed * kThreads + sh.threads[i % listed];
-        if (v >= s.vecs) continue;
-        const uint4 x = load16(vec0 + int64_t(v) * 16);
-        if (order_of(V::top(x)) < least) continue;
-#pragma unroll
-        for (int e = 0; e < V::kN / 2; ++e) {
-          const float2 f = V::two(x, e);
-          offer(f.x, first_vec + v * V::kN + 2 * e);
-          offer(f.y, first_vec + v * V::kN + 2 * e + 1);
-        }
-      }
-      if (tid < s.head) offer(V::one(s.row + int64_t(s.first + tid) * V::kBytes), s.first + tid);
-      if (tid < s.tail) {
-        const int col = first_vec + s.vecs * V::kN + tid;
-        offer(V::one(s.row + int64_t(col) * V::kBytes), col);
-      }
-      __syncthreads();
-    };
-    collect(bound);
+    collect<DTYPE>(sh, sh, s, sh.listed, bound);
+    __syncthreads();
     int n = sh.found;
     if (n > kCandidates) {
       // more equal values than the list holds: those above the bound, then the lowest columns
@@ -298,7 +343,8 @@ __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
       __syncthreads();
       if (tid == 0) sh.found = 0;
       __syncthreads();
-      collect(bound + 1);
+      collect<DTYPE>(sh, sh, s, sh.listed, bound + 1);
+      __syncthreads();
       n = sh.found;
       one_by_one = n > kCandidates;
       if (n < k) {
@@ -311,7 +357,7 @@ __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
           if (lane == 0) sh.warp_count[warp] = __popc(ties);
           __syncthreads();
           int before = 0, total = 0;
-          for (int w = 0; w < kThreads / 32; ++w) {
+          for (int w = 0; w < kWarps; ++w) {
             before += w < warp ? sh.warp_count[w] : 0;
             total += sh.warp_count[w];
           }
@@ -323,7 +369,7 @@ __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
         }
       }
     }
-    if (!one_by_one) rank_candidates(sh, n, k);
+    if (!one_by_one) rank_keys(sh, sh.cand, n, k);
   }
   if (one_by_one) {
     // NaNs, or too many values above the bound: one after the other
@@ -353,8 +399,58 @@ __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
   __syncthreads();
 }
 
+// What one thread has seen of its columns.
 template <int DTYPE>
-__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+struct Running {
+  using V = Vec<DTYPE>;
+  f32x2 sum[2] = {0, 0}, prod[2] = {0, 0};
+  float m = -INFINITY;      // largest value that the reference was taken from
+  float r = -INFINITY;      // fl(m log2 e)
+  float top = -INFINITY;    // largest value at all, or NaN
+
+  template <int N>
+  __device__ __forceinline__ void take(const uint4 (&x)[N]) {
+    float t = V::top(x[0]);
+#pragma unroll
+    for (int j = 1; j < N; ++j) t = max_nan(t, V::top(x[j]));
+    top = max_nan(top, t);
+    if (!(t >= V::kLow)) return;        // nothing here that counts beside a higher value
+    if (t > m) {
+      m = t;
+      const float next = t * kLog2e, d = fmaxf(r - next, kFloor);
+      const float f = exp2_fast(d);
+      const f32x2 dd = pair(d, d), ff = pair(f, f);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        prod[i] = mul2(fma2(dd, sum[i], prod[i]), ff);
+        sum[i] = mul2(sum[i], ff);
+      }
+      r = next;
+    }
+    const f32x2 ref = pair(-r, -r), scale = pair(kLog2e, kLog2e);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint4 c = V::clamp(x[j]);
+#pragma unroll
+      for (int e = 0; e < V::kN / 2; ++e) {
+        const float2 f = V::two(c, e);
+        const f32x2 y = fma2(pair(f.x, f.y), scale, ref);
+        const float2 yy = halves(y);
+        const f32x2 w = pair(exp2_fast(yy.x), exp2_fast(yy.y));
+        sum[e % 2] = add2(sum[e % 2], w);
+        prod[e % 2] = fma2(y, w, prod[e % 2]);
+      }
+    }
+  }
+
+  __device__ __forceinline__ Sums sums() const {
+    const float2 s0 = halves(add2(sum[0], sum[1])), u0 = halves(add2(prod[0], prod[1]));
+    return Sums{r, s0.x + s0.y, u0.x + u0.y, top};
+  }
+};
+
+template <int DTYPE>
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
   using V = Vec<DTYPE>;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -363,7 +459,10 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const __gri
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const char *row = a.logits + r * a.ld * V::kBytes;
   const Slice s = slice_of<DTYPE>(row, a.vocab, rank, ctas);
-  const char *vec0 = row + int64_t(s.first + s.head) * V::kBytes;
+  const auto meet = [&]() {        // the row's CTAs, or this one's threads
+    if (ctas > 1) cluster.sync();
+    else __syncthreads();
+  };
 
   // the token's logit is wanted last: ask for it first
   long long token = -1;
@@ -372,131 +471,144 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const __gri
     token = a.tokens[r];
     if (token >= 0 && token < a.vocab) given = V::one(row + token * V::kBytes);
   }
+  if (tid == 0) sh.listed = sh.found = sh.slow = 0;
 
-  Sums mine = {-INFINITY, 0.f, 0.f};
+  // ---- the pass: kUnroll vectors per thread at a time, the next ones on their way
+  Sums mine;
   {
-    f32x2 sum[2] = {0, 0}, prod[2] = {0, 0};
+    Running<DTYPE> run;
+    const char *p = row + int64_t(s.first + s.head) * V::kBytes + tid * 16;
+    const int whole = s.vecs / (kUnroll * kThreads);        // turns without a bound to check
+    int left = s.vecs - whole * (kUnroll * kThreads) - tid; // of the last turn, for this thread
     uint4 next[kUnroll];
+    const auto fetch_whole = [&]() {
 #pragma unroll
-    for (int j = 0; j < kUnroll; ++j) {
-      const int v = j * kThreads + tid;
-      next[j] = v < s.vecs ? load16(vec0 + int64_t(v) * 16) : V::none();
-    }
-    for (int v0 = 0; v0 < s.vecs; v0 += kUnroll * kThreads) {
+      for (int j = 0; j < kUnroll; ++j) next[j] = load16(p + j * (kThreads * 16));
+      p += kUnroll * kThreads * 16;
+    };
+    const auto fetch_last = [&]() {
+#pragma unroll
+      for (int j = 0; j < kUnroll; ++j) next[j] = j * kThreads < left ? load16(p + j * (kThreads * 16)) : V::none();
+    };
+    if (whole > 0) fetch_whole();
+    else fetch_last();
+    for (int i = 0; i < whole; ++i) {
       uint4 x[kUnroll];
 #pragma unroll
-      for (int j = 0; j < kUnroll; ++j) {
-        x[j] = next[j];
-        const int v = v0 + (kUnroll + j) * kThreads + tid;
-        next[j] = v < s.vecs ? load16(vec0 + int64_t(v) * 16) : V::none();
-      }
-      float top = V::top(x[0]);
-#pragma unroll
-      for (int j = 1; j < kUnroll; ++j) top = max_nan(top, V::top(x[j]));
-      if (!(top <= mine.m)) {
-        const float d = fmaxf((mine.m - top) * kLog2e, kFloor);
-        const f32x2 dd = pair(d, d), f = pair(exp2_fast(d), exp2_fast(d));
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          prod[i] = mul2(fma2(dd, sum[i], prod[i]), f);
-          sum[i] = mul2(sum[i], f);
-        }
-        mine.m = top;
-      }
-      const float ref = mine.m == -INFINITY ? 0.f : -mine.m;
-      const f32x2 ref2 = pair(ref, ref), scale = pair(kLog2e, kLog2e);
-#pragma unroll
-      for (int j = 0; j < kUnroll; ++j)
-#pragma unroll
-        for (int e = 0; e < V::kN / 2; ++e) {
-          const float2 f = V::two(x[j], e);
-          const float2 y = halves(mul2(add2(pair(f.x, f.y), ref2), scale));
-          const float y0 = fmaxf(y.x, kFloor), y1 = fmaxf(y.y, kFloor);
-          const f32x2 w = pair(exp2_fast(y0), exp2_fast(y1));
-          sum[e % 2] = add2(sum[e % 2], w);
-          prod[e % 2] = fma2(pair(y0, y1), w, prod[e % 2]);
-        }
+      for (int j = 0; j < kUnroll; ++j) x[j] = next[j];
+      if (i + 1 < whole) fetch_whole();
+      else fetch_last();
+      run.take(x);
     }
-    const float2 s0 = halves(add2(sum[0], sum[1])), u0 = halves(add2(prod[0], prod[1]));
-    mine.s = s0.x + s0.y;
-    mine.u = u0.x + u0.y;
+    run.take(next);
+    mine = run.sums();
   }
   // the single columns at the ends: one per thread
   const auto single = [&](int col) {
     const float x = V::one(row + int64_t(col) * V::kBytes);
-    join(mine, Sums{x, x == -INFINITY ? 0.f : 1.f, 0.f});
+    join(mine, x >= V::kLow ? Sums{x * kLog2e, 1.f, 0.f, x} : Sums{-INFINITY, 0.f, 0.f, x});
   };
   if (tid < s.head) single(s.first + tid);
   if (tid < s.tail) single(s.first + s.head + s.vecs * V::kN + tid);
 
+  // ---- sums and bounds of the threads, together
+  const uint32_t order = order_of(mine.top);
+  const int span = min(32, kThreads / kGroups * ctas);     // threads per group: 64 groups a row, or 128
+  const int parts = kThreads / span;
+  if (a.top > 0) {
+    uint32_t g = mine.top != mine.top ? 0xffffffffu : order;    // (a NaN is no order's: it shows)
+#pragma unroll
+    for (int x = 1; x < 32; x *= 2)
+      if (x < span) g = max(g, __shfl_xor_sync(~0u, g, x));
+    if (tid % span == 0) sh.part[tid / span] = g;
+  }
   Sums all = mine;
 #pragma unroll
-  for (int x = 16; x; x /= 2) {
-    Sums o;
-    o.m = __shfl_xor_sync(~0u, all.m, x);
-    o.s = __shfl_xor_sync(~0u, all.s, x);
-    o.u = __shfl_xor_sync(~0u, all.u, x);
-    join(all, o);
-  }
+  for (int x = 16; x; x /= 2) join(all, shuffled(all, x));
   if (lane == 0) sh.warp[warp] = all;
-  if (a.top > 0) top_of_slice<DTYPE>(sh, s, mine.m, a.top);
-  else __syncthreads();
-  if (warp == 0) {
-    all = lane < kThreads / 32 ? sh.warp[lane] : Sums{-INFINITY, 0.f, 0.f};
+  meet();
+  if (rank == 0 && warp == kWarps - 1) {
+    all = kNoSums;
+    for (int i = lane; i < ctas * kWarps; i += 32)
+      join(all, ctas > 1 ? cluster.map_shared_rank(&sh, i / kWarps)->warp[i % kWarps] : sh.warp[i]);
 #pragma unroll
-    for (int x = kThreads / 64; x; x /= 2) {
-      Sums o;
-      o.m = __shfl_xor_sync(~0u, all.m, x);
-      o.s = __shfl_xor_sync(~0u, all.s, x);
-      o.u = __shfl_xor_sync(~0u, all.u, x);
-      join(all, o);
+    for (int x = 16; x; x /= 2) join(all, shuffled(all, x));
+    if (lane == 0) sh.row = all;
+  }
+  if (a.top > 0) {
+    Shared *leader = ctas > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+    const int groups = parts * ctas;
+    uint32_t g = 0;
+    if (tid < groups) {
+      g = ctas > 1 ? cluster.map_shared_rank(&sh, tid / parts)->part[tid % parts] : sh.part[tid];
+      sh.group[tid] = g;
+      if (g == 0xffffffffu) sh.slow = 1;
     }
-    if (lane == 0) sh.all = all;
+    if (tid < kMaxTop) sh.top[tid] = 0;
+    __syncthreads();
+    if (tid < groups) {
+      int above = 0;
+      for (int j = 0; j < groups; ++j) above += sh.group[j] > g || (sh.group[j] == g && j < tid);
+      if (above == a.top - 1) sh.bound = g;
+    }
+    bool slow = sh.slow != 0;
+    __syncthreads();
+    if (!slow) {
+      const uint32_t bound = sh.bound;
+      if (order >= bound) sh.threads[atomicAdd(&sh.listed, 1)] = tid;
+      __syncthreads();
+      collect<DTYPE>(sh, *leader, s, sh.listed, bound);
+    }
+    meet();
+    const int n = leader->found;
+    if (slow || n > kCandidates) {
+      // (all CTAs of the row see the same)
+      meet();          // everybody has read `found`
+      top_of_slice<DTYPE>(sh, s, mine.top, a.top);
+      meet();
+      if (rank == 0) {
+        for (int i = tid; i < ctas * a.top; i += kThreads)
+          sh.merged[i] = ctas > 1 ? cluster.map_shared_rank(&sh, i / a.top)->top[i % a.top] : sh.top[i];
+        __syncthreads();
+        rank_keys(sh, sh.merged, ctas * a.top, a.top);
+      }
+    } else if (rank == 0) {
+      rank_keys(sh, sh.cand, n, a.top);
+    }
+  }
+  if (ctas > 1) {
+    cluster.sync();          // nobody leaves while its shared memory is read
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
   }
 
-  // ---- join the cluster
-  if (ctas > 1) {
-    cluster.sync();
-    if (rank == 0) {
-      if (warp == 0) {
-        all = lane < ctas ? cluster.map_shared_rank(&sh, lane)->all : Sums{-INFINITY, 0.f, 0.f};
-#pragma unroll
-        for (int x = kMaxCluster / 2; x; x /= 2) {
-          Sums o;
-          o.m = __shfl_xor_sync(~0u, all.m, x);
-          o.s = __shfl_xor_sync(~0u, all.s, x);
-          o.u = __shfl_xor_sync(~0u, all.u, x);
-          join(all, o);
-        }
-      }
-      for (int i = tid; i < ctas * a.top; i += kThreads)
-        sh.merged[i] = cluster.map_shared_rank(&sh, i / a.top)->top[i % a.top];
-    }
-    cluster.sync();        // nobody leaves while its shared memory is read
-    if (rank != 0) return;
-    if (warp == 0 && lane == 0) sh.all = all;
+  // ---- results
+  all = sh.row;
+  const bool bad = !(all.top < INFINITY);               // a NaN or +infinity in the row
+  const bool empty = all.top == -INFINITY;
+  const bool ends = !bad && !empty && (all.top < V::kLow || all.top > kHigh);   // weights of 0 and 1
+  if (ends) {
+    if (tid == 0) sh.found = 0;
     __syncthreads();
-    unsigned long long key = 0;
-    int above = kMaxTop;
-    if (tid < ctas * a.top && (key = sh.merged[tid]) != 0) {
-      above = 0;
-      for (int j = 0; j < ctas * a.top; ++j) above += sh.merged[j] > key;
-    }
-    if (above < a.top) sh.top[above] = key;
+    int count = 0;
+    for (int i = tid; i < a.vocab; i += kThreads) count += V::one(row + int64_t(i) * V::kBytes) == all.top;
+    atomicAdd(&sh.found, count);
+    __syncthreads();
+    all.s = float(sh.found);
+    all.u = 0.f;
   }
-  __syncthreads();
-  all = sh.all;
-  const bool bad = !(all.m < INFINITY);                 // a NaN or +infinity in the row
-  const bool empty = all.m == -INFINITY;
-  const float log_s = log2f(all.s) * kLn2;
+  const float log2_s = log2f(all.s);
+  // log p of the most probable column; the others lie x - max below it
+  const float peak = kLn2 * ((ends ? 0.f : fmaf(all.top, kLog2e, -all.r)) - log2_s);
   const auto logp = [&](float x) {
     if (bad) return NAN;
     if (empty || x == -INFINITY) return -INFINITY;
-    return x - all.m - log_s;
+    return (x - all.top) + peak;
   };
   if (tid == 0) {
     a.logprob[r] = token >= 0 && token < a.vocab ? logp(given) : bad ? NAN : -INFINITY;
-    a.entropy[r] = bad ? NAN : empty ? 0.f : kLn2 * (log2f(all.s) - all.u / all.s);
+    a.entropy[r] = bad ? NAN : empty ? 0.f : fmaxf(0.f, kLn2 * (log2_s - all.u / all.s));
   }
   if (tid < a.top) {
     const unsigned long long key = sh.top[tid];
@@ -505,11 +617,11 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const __gri
   }
 }
 
-// CTAs per row: as many as fill the device a few times over, none with less than about one
-// vector per thread.
+// CTAs per row: as many as are resident at once (four per SM), none with less than about two
+// vectors per thread.
 int cluster_size(int rows, int vocab, int sms) {
   int c = 1;
-  while (c < kMaxCluster && int64_t(rows) * c < 4 * int64_t(sms) && vocab / (2 * c) >= 4096) c *= 2;
+  while (c < kMaxCluster && int64_t(rows) * 2 * c <= 4 * int64_t(sms) && vocab / (2 * c) >= 4096) c *= 2;
   return c;
 }
 
