@@ -13,8 +13,9 @@
 // counted instead.
 //
 // The top alternatives cost the pass nothing.  Its running maxima, one per thread, give a bound:
-// the k-th largest maximum of 64 groups of threads is at most the k-th largest logit.  Only the
-// columns of the threads whose own maximum reaches the bound (little more than k) are read
+// the k-th largest maximum of 64 groups of threads is at most the k-th largest logit.  Each turn
+// of the pass also leaves its maximum per thread in shared memory (16 bits, rounded so that
+// nothing is missed); only the turns that reach the bound, little more than k, are read
 // again, from L2, and what reaches the bound there is ranked.  Rows full of equal values (a mask
 // that leaves less than k columns) overflow that list; they take the slow way: the logits above
 // the bound and then the lowest columns that equal it.
@@ -35,12 +36,12 @@ namespace ypk {
 namespace {
 
 constexpr int kMaxTop = 32;
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kGroups = 64;        // of 4 threads: what the bound of a slice's top list is taken from
+constexpr int kGroups = 64;        // of threads: what the bound of a top list is taken from
 constexpr int kMaxGroups = 128;    // over a cluster
 constexpr int kCandidates = 1024;
 constexpr int kUnroll = 4;         // 16-byte loads in flight per thread (and as many ahead)
+constexpr int kSlots = 32;         // remembered turns of the pass (several share one beyond that)
+constexpr int kMaxEntries = 512;   // (thread, slot) pairs to be read again
 constexpr int kMaxCluster = 16;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
@@ -224,20 +225,22 @@ __device__ __forceinline__ Sums shuffled(const Sums &a, int x) {
   return o;
 }
 
-struct Shared {
-  Sums warp[kWarps];
+template <int THREADS>
+struct SharedOf {
+  Sums warp[THREADS / 32];
   Sums row;                               // of the whole row
-  uint32_t part[kGroups];                 // maxima of this CTA's groups of threads
-  uint32_t group[kMaxGroups];             // of the row's
+  alignas(16) uint32_t part[kGroups];     // maxima of this CTA's groups of threads
+  alignas(16) uint32_t group[kMaxGroups]; // of the row's
   uint32_t bound;
   int slow;                               // the row has a NaN, or too many candidates
   int listed, found;
-  int threads[kThreads];                  // whose columns are read again
+  uint32_t entry[kMaxEntries];            // slot << 16 | thread: columns to be read again
+  uint16_t slot_max[kSlots][THREADS];    // upper half of the order of a turn's maximum
   unsigned long long cand[kCandidates];
   unsigned long long top[kMaxTop];        // falling; 0: none
   unsigned long long best;
   unsigned long long merged[kMaxCluster * kMaxTop];
-  int warp_count[kWarps];
+  int warp_count[THREADS / 32];
 };
 
 // The columns of one CTA: a few single ones, whole 16-byte vectors, a few single ones.
@@ -264,8 +267,9 @@ __device__ __forceinline__ Slice slice_of(const char *row, int vocab, int rank, 
 }
 
 // The k largest of n keys in order into sh.top; every thread calls.
-__device__ void rank_keys(Shared &sh, const unsigned long long *keys, int n, int k) {
-  for (int i = threadIdx.x; i < n; i += kThreads) {
+template <int THREADS>
+__device__ void rank_keys(SharedOf<THREADS> &sh, const unsigned long long *keys, int n, int k) {
+  for (int i = threadIdx.x; i < n; i += THREADS) {
     const unsigned long long mine = keys[i];
     if (mine == 0) continue;
     int above = 0;
@@ -274,30 +278,42 @@ __device__ void rank_keys(Shared &sh, const unsigned long long *keys, int n, int
   }
 }
 
+// Lists the slots of this thread that reach the bound.
+template <int THREADS>
+__device__ __forceinline__ void list_slots(SharedOf<THREADS> &sh, int slots, uint32_t bound) {
+  for (int i = 0; i < slots; ++i)
+    if (sh.slot_max[i][threadIdx.x] >= bound >> 16) {
+      const int at = atomicAdd(&sh.listed, 1);
+      if (at < kMaxEntries) sh.entry[at] = uint32_t(i) << 16 | threadIdx.x;
+    }
+}
+
 // Puts the columns of this CTA's slice that are at least `least` in order into the list of `to`
-// (counted in to.found, as far as there is room), from the threads of sh.threads.
-template <int DTYPE>
-__device__ __forceinline__ void collect(Shared &sh, Shared &to, const Slice &s, int listed, uint32_t least) {
+// (counted in to.found, as far as there is room), from the listed slots of `each` vectors.
+template <int DTYPE, int THREADS>
+__device__ __forceinline__ void collect(SharedOf<THREADS> &sh, SharedOf<THREADS> &to, const Slice &s, int listed,
+                                        int each, uint32_t least) {
   using V = Vec<DTYPE>;
+  constexpr int kThreads = THREADS;
   const int tid = threadIdx.x, first_vec = s.first + s.head;
   const char *vec0 = s.row + int64_t(first_vec) * V::kBytes;
-  const int rounds = (s.vecs + kThreads - 1) / kThreads;
   const auto offer = [&](float x, int col) {
     const uint32_t o = order_of(x);
     if (o < least) return;
     const int at = atomicAdd(&to.found, 1);
     if (at < kCandidates) to.cand[at] = key_of(o, uint32_t(col));
   };
-  for (int i = tid; i < listed * rounds; i += kThreads) {
-    const int v = i / listed * kThreads + sh.threads[i % listed];
+  for (int i = tid; i < listed * each; i += kThreads) {
+    const uint32_t e = sh.entry[i % listed];
+    const int v = (int(e >> 16) * each + i / listed) * kThreads + int(e & 0xffffu);
     if (v >= s.vecs) continue;
     const uint4 x = load16(vec0 + int64_t(v) * 16);
     if (order_of(V::top(x)) < least) continue;
 #pragma unroll
-    for (int e = 0; e < V::kN / 2; ++e) {
-      const float2 f = V::two(x, e);
-      offer(f.x, first_vec + v * V::kN + 2 * e);
-      offer(f.y, first_vec + v * V::kN + 2 * e + 1);
+    for (int k = 0; k < V::kN / 2; ++k) {
+      const float2 f = V::two(x, k);
+      offer(f.x, first_vec + v * V::kN + 2 * k);
+      offer(f.y, first_vec + v * V::kN + 2 * k + 1);
     }
   }
   if (tid < s.head) offer(V::one(s.row + int64_t(s.first + tid) * V::kBytes), s.first + tid);
@@ -307,10 +323,29 @@ __device__ __forceinline__ void collect(Shared &sh, Shared &to, const Slice &s, 
   }
 }
 
+// The k-th largest of n group maxima, or a little less: the lower bits make way for the group's
+// number, so that no two are alike.  Every thread calls; sh.bound is there after a barrier.
+template <int THREADS>
+__device__ __forceinline__ void find_bound(SharedOf<THREADS> &sh, int n, int k) {
+  const int tid = threadIdx.x;
+  if (tid >= n) return;
+  const uint32_t mine = sh.group[tid];
+  int above = 0;
+  for (int j = 0; j < n; j += 4) {
+    const uint4 g = *reinterpret_cast<const uint4 *>(sh.group + j);
+    above += (g.x > mine) + (g.y > mine) + (g.z > mine) + (g.w > mine);
+  }
+  if (above == k - 1) sh.bound = mine & ~uint32_t(kMaxGroups - 1);
+}
+__device__ __forceinline__ uint32_t group_key(uint32_t order, int group) {
+  return (order & ~uint32_t(kMaxGroups - 1)) | uint32_t(group);
+}
+
 // The slow way: the k largest of this CTA's slice, exactly, into sh.top.
-template <int DTYPE>
-__device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
+template <int DTYPE, int THREADS>
+__device__ __forceinline__ void top_of_slice(SharedOf<THREADS> &sh, const Slice &s, float my_max, int k) {
   using V = Vec<DTYPE>;
+  constexpr int kThreads = THREADS, kWarps = THREADS / 32;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int columns = s.head + s.vecs * V::kN + s.tail;
   const uint32_t mine = order_of(my_max);
@@ -325,16 +360,18 @@ __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
   bool one_by_one = __syncthreads_or(my_max != my_max);
   if (!one_by_one) {
     if (tid < kGroups) {
-      const uint32_t gi = sh.group[tid];      // thread i ranks group i
+      // a bound that is one of the values: ties are told from what is above
+      const uint32_t gi = sh.group[tid];
       int above = 0;
       for (int j = 0; j < kGroups; ++j) above += sh.group[j] > gi || (sh.group[j] == gi && j < tid);
       if (above == k - 1) sh.bound = gi;
     }
     __syncthreads();
     const uint32_t bound = sh.bound;
-    if (mine >= bound) sh.threads[atomicAdd(&sh.listed, 1)] = tid;
+    if (mine >= bound) sh.entry[atomicAdd(&sh.listed, 1)] = tid;      // all of its vectors: one slot
     __syncthreads();
-    collect<DTYPE>(sh, sh, s, sh.listed, bound);
+    const int listed = sh.listed, rounds = (s.vecs + kThreads - 1) / kThreads;
+    collect<DTYPE, THREADS>(sh, sh, s, listed, rounds, bound);
     __syncthreads();
     int n = sh.found;
     if (n > kCandidates) {
@@ -343,7 +380,7 @@ __device__ void top_of_slice(Shared &sh, const Slice &s, float my_max, int k) {
       __syncthreads();
       if (tid == 0) sh.found = 0;
       __syncthreads();
-      collect<DTYPE>(sh, sh, s, sh.listed, bound + 1);
+      collect<DTYPE, THREADS>(sh, sh, s, listed, rounds, bound + 1);
       __syncthreads();
       n = sh.found;
       one_by_one = n > kCandidates;
@@ -409,12 +446,12 @@ struct Running {
   float top = -INFINITY;    // largest value at all, or NaN
 
   template <int N>
-  __device__ __forceinline__ void take(const uint4 (&x)[N]) {
+  __device__ __forceinline__ float take(const uint4 (&x)[N]) {      // the largest of x
     float t = V::top(x[0]);
 #pragma unroll
     for (int j = 1; j < N; ++j) t = max_nan(t, V::top(x[j]));
     top = max_nan(top, t);
-    if (!(t >= V::kLow)) return;        // nothing here that counts beside a higher value
+    if (!(t >= V::kLow)) return t;      // nothing here that counts beside a higher value
     if (t > m) {
       m = t;
       const float next = t * kLog2e, d = fmaxf(r - next, kFloor);
@@ -441,6 +478,7 @@ struct Running {
         prod[e % 2] = fma2(y, w, prod[e % 2]);
       }
     }
+    return t;
   }
 
   __device__ __forceinline__ Sums sums() const {
@@ -449,9 +487,11 @@ struct Running {
   }
 };
 
-template <int DTYPE>
-__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
+template <int DTYPE, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
   using V = Vec<DTYPE>;
+  using Shared = SharedOf<THREADS>;
+  constexpr int kThreads = THREADS, kWarps = THREADS / 32;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = int(cluster.num_blocks()), rank = int(cluster.block_rank());
@@ -475,10 +515,22 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
 
   // ---- the pass: kUnroll vectors per thread at a time, the next ones on their way
   Sums mine;
+  const int turns = s.vecs / (kUnroll * kThreads) + 1;               // the last one has bounds to check
+  const int turns_per_slot = (turns + kSlots - 1) / kSlots;
   {
     Running<DTYPE> run;
     const char *p = row + int64_t(s.first + s.head) * V::kBytes + tid * 16;
-    const int whole = s.vecs / (kUnroll * kThreads);        // turns without a bound to check
+    const int whole = turns - 1;
+    float slot_top = -INFINITY;
+    int slot = 0, in_slot = 0;
+    const auto remember = [&](float t) {
+      if (!TOP) return;
+      slot_top = fmaxf(slot_top, t);
+      if (++in_slot < turns_per_slot) return;
+      sh.slot_max[slot++][tid] = uint16_t(order_of(slot_top) >> 16);
+      slot_top = -INFINITY;
+      in_slot = 0;
+    };
     int left = s.vecs - whole * (kUnroll * kThreads) - tid; // of the last turn, for this thread
     uint4 next[kUnroll];
     const auto fetch_whole = [&]() {
@@ -498,9 +550,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
       for (int j = 0; j < kUnroll; ++j) x[j] = next[j];
       if (i + 1 < whole) fetch_whole();
       else fetch_last();
-      run.take(x);
+      remember(run.take(x));
     }
-    run.take(next);
+    remember(run.take(next));
+    if (TOP && in_slot > 0) sh.slot_max[slot][tid] = uint16_t(order_of(slot_top) >> 16);
     mine = run.sums();
   }
   // the single columns at the ends: one per thread
@@ -515,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   const uint32_t order = order_of(mine.top);
   const int span = min(32, kThreads / kGroups * ctas);     // threads per group: 64 groups a row, or 128
   const int parts = kThreads / span;
-  if (a.top > 0) {
+  if (TOP) {
     uint32_t g = mine.top != mine.top ? 0xffffffffu : order;    // (a NaN is no order's: it shows)
 #pragma unroll
     for (int x = 1; x < 32; x *= 2)
@@ -527,44 +580,46 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   for (int x = 16; x; x /= 2) join(all, shuffled(all, x));
   if (lane == 0) sh.warp[warp] = all;
   meet();
-  if (rank == 0 && warp == kWarps - 1) {
+  // the last warp joins the row's sums, beside the others' reading
+  const auto join_row = [&]() {
+    if (rank != 0 || warp != kWarps - 1) return;
     all = kNoSums;
     for (int i = lane; i < ctas * kWarps; i += 32)
       join(all, ctas > 1 ? cluster.map_shared_rank(&sh, i / kWarps)->warp[i % kWarps] : sh.warp[i]);
 #pragma unroll
     for (int x = 16; x; x /= 2) join(all, shuffled(all, x));
     if (lane == 0) sh.row = all;
-  }
-  if (a.top > 0) {
-    Shared *leader = ctas > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+  };
+  if (!TOP) join_row();
+  if (TOP) {
+    Shared *leader = rank > 0 ? cluster.map_shared_rank(&sh, 0) : &sh;
     const int groups = parts * ctas;
     uint32_t g = 0;
     if (tid < groups) {
       g = ctas > 1 ? cluster.map_shared_rank(&sh, tid / parts)->part[tid % parts] : sh.part[tid];
-      sh.group[tid] = g;
+      sh.group[tid] = group_key(g, tid);
       if (g == 0xffffffffu) sh.slow = 1;
     }
     if (tid < kMaxTop) sh.top[tid] = 0;
     __syncthreads();
-    if (tid < groups) {
-      int above = 0;
-      for (int j = 0; j < groups; ++j) above += sh.group[j] > g || (sh.group[j] == g && j < tid);
-      if (above == a.top - 1) sh.bound = g;
-    }
-    bool slow = sh.slow != 0;
+    find_bound(sh, groups, a.top);
+    const bool slow = sh.slow != 0;
     __syncthreads();
     if (!slow) {
       const uint32_t bound = sh.bound;
-      if (order >= bound) sh.threads[atomicAdd(&sh.listed, 1)] = tid;
+      if (order >= bound) list_slots(sh, (turns + turns_per_slot - 1) / turns_per_slot, bound);
       __syncthreads();
-      collect<DTYPE>(sh, *leader, s, sh.listed, bound);
+      const int listed = sh.listed;
+      if (listed <= kMaxEntries) collect<DTYPE, THREADS>(sh, *leader, s, listed, turns_per_slot * kUnroll, bound);
+      else if (tid == 0) atomicAdd(&leader->found, kCandidates + 1);      // too many: the slow way
     }
+    join_row();
     meet();
     const int n = leader->found;
     if (slow || n > kCandidates) {
       // (all CTAs of the row see the same)
       meet();          // everybody has read `found`
-      top_of_slice<DTYPE>(sh, s, mine.top, a.top);
+      top_of_slice<DTYPE, THREADS>(sh, s, mine.top, a.top);
       meet();
       if (rank == 0) {
         for (int i = tid; i < ctas * a.top; i += kThreads)
@@ -610,21 +665,48 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     a.logprob[r] = token >= 0 && token < a.vocab ? logp(given) : bad ? NAN : -INFINITY;
     a.entropy[r] = bad ? NAN : empty ? 0.f : fmaxf(0.f, kLn2 * (log2_s - all.u / all.s));
   }
-  if (tid < a.top) {
+  if (TOP && tid < a.top) {
     const unsigned long long key = sh.top[tid];
     a.top_token[r * a.top + tid] = 0xffffffffu - uint32_t(key);
     a.top_logprob[r * a.top + tid] = logp(value_of(uint32_t(key >> 32)));
   }
 }
 
-// CTAs per row: as many as are resident at once (four per SM), none with less than about two
-// vectors per thread.
+// CTAs per row: up to three per SM in all, none with less than about two vectors per thread.
 int cluster_size(int rows, int vocab, int sms) {
   int c = 1;
-  while (c < kMaxCluster && int64_t(rows) * 2 * c <= 4 * int64_t(sms) && vocab / (2 * c) >= 4096) c *= 2;
+  while (c < kMaxCluster && int64_t(rows) * 2 * c <= 3 * int64_t(sms) && vocab / (2 * c) >= 4096) c *= 2;
   return c;
 }
 
+template <int DTYPE, bool TOP, int THREADS>
+int launch_shape(const LogprobArgs &a, int rows, int device, int sms, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};      // devices where clusters of sixteen have been asked for
+  auto *kernel = token_logprobs_kernel<DTYPE, TOP, THREADS>;
+  cudaError_t e = cudaSuccess;
+  if (!(ready.load(std::memory_order_relaxed) >> device & 1)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: set-up: %s", cudaGetErrorString(e));
+    ready.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+  }
+  const int c = cluster_size(rows, a.vocab, sms);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(rows) * c);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: launch: %s", cudaGetErrorString(e));
+  return YPK_OK;
+}
+
+// With alternatives wanted and more rows than 256-thread CTAs are resident, CTAs of 128 threads:
+// their phases without loads overlap with more others'.
 template <int DTYPE>
 int launch_logprobs(const LogprobArgs &a, int rows, cudaStream_t st) {
   static std::atomic<int> sms_of[64];
@@ -635,25 +717,12 @@ int launch_logprobs(const LogprobArgs &a, int rows, cudaStream_t st) {
   int sms = sms_of[device].load(std::memory_order_relaxed);
   if (!sms) {
     e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess)   // clusters of sixteen are an option that has to be asked for
-      e = cudaFuncSetAttribute(token_logprobs_kernel<DTYPE>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: set-up: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: SM count: %s", cudaGetErrorString(e));
     sms_of[device].store(sms, std::memory_order_relaxed);
   }
-  const int c = cluster_size(rows, a.vocab, sms);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(rows) * c);
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = c;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DTYPE>, a);
-  if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: launch: %s", cudaGetErrorString(e));
-  return YPK_OK;
+  if (!a.top) return launch_shape<DTYPE, false, 256>(a, rows, device, sms, st);
+  return rows > 4 * sms ? launch_shape<DTYPE, true, 128>(a, rows, device, sms, st)
+                        : launch_shape<DTYPE, true, 256>(a, rows, device, sms, st);
 }
 
 }  // namespace
