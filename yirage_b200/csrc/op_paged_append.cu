@@ -1,5 +1,8 @@
 // New tokens' K and V rows into a paged cache, with RMS norm and rotation on the way
 // (ypk_paged_append), and the host checks that the paged-cache operators share.
+#include <algorithm>
+#include <initializer_list>
+
 #include "op_paged.h"
 
 namespace ypk {
@@ -62,8 +65,13 @@ struct AppendArgs {
   int64_t q_token, q_group, q_head, o_token, o_group, o_head;
   int64_t table_stride;
   int tokens, q_heads, group, rot, max_pos;
+  int rows_per_cta, heads_per_cta;
+  FastDivisor heads_div, group_div;
   float eps;
 };
+
+constexpr int kAppendThreads = 128;
+constexpr int kMaxRows = 8;          // tokens per CTA
 
 // Eight table values as floats, from 16 or 32 bits.
 template <class T, bool WIDE_TABLE>
@@ -77,120 +85,179 @@ __device__ __forceinline__ void load_table(const char *base, int64_t element, fl
   }
 }
 
-// One (token, head) per D / 16 threads; each thread holds two chunks of eight dimensions: the
-// pair that a rotation mixes, or two neighbours behind the rotated part.
+// Where one new token goes.
+struct Place {
+  int64_t slot;    // element offset of its row for K/V head 0; -1: nowhere
+  int64_t table;   // element offset of its row in the rotary tables
+};
+
+// The place of row `row`, found by a whole warp.  Broken entries are reported and give slot -1.
+__device__ __forceinline__ Place find_place(const AppendArgs &a, int row) {
+  const int lane = threadIdx.x % 32;
+  // the request whose rows hold this one: rounds of 32 evenly spaced looks at the row offsets
+  int lo = 0, n = a.c.num_requests;      // the answer is among requests lo .. lo + n
+  while (n > 0) {
+    const int step = (n + 31) / 32, at = lo + (lane + 1) * step;     // requests lo .. at - 1 end before?
+    const bool before = at <= lo + n && __ldg(a.c.qo + at) <= row;
+    const int skip = __popc(__ballot_sync(~0u, before)) * step;
+    lo += skip;
+    n = min(n - skip, step - 1);
+  }
+  Place p = {-1, 0};
+  if (lo >= a.c.num_requests) return p;                              // a padding row
+  const PagedRun run = paged_run(__ldg(a.c.indptr + lo), __ldg(a.c.indptr + lo + 1), __ldg(a.c.last + lo),
+                                 a.c.page_size, a.c.num_indices);
+  const int64_t pos = paged_new_position(run, __ldg(a.c.qo + lo + 1), row);
+  int bad = 0;
+  if (run.broken) bad = kPagedBadTable;
+  else if (__ldg(a.c.qo + lo) > row || pos < 0 || pos >= run.tokens) bad = kPagedBadLength;
+  else if (a.cos && pos >= a.max_pos) bad = kPagedBadPosition;
+  else {
+    const int page = __ldg(a.c.indices + run.first + int(pos) / a.c.page_size);
+    p.slot = paged_row(page, a.c.num_pages, pos, a.c.page_size, a.c.stride_page, a.c.stride_token);
+    p.table = pos * a.table_stride;
+    if (p.slot < 0) bad = kPagedBadPage;
+  }
+  if (bad && lane == 0) paged_flag(a.c, bad);
+  return p;
+}
+
+// A CTA takes a.rows_per_cta tokens and, of each, the heads of blockIdx.y's share.  Its warps look
+// up where the tokens go; then D / 16 threads move one (token, head), each two chunks of eight
+// dimensions: the pair that a rotation mixes, or two neighbours behind the rotated part.  Four
+// (token, head)s per thread are read before the first is finished, the first four before the
+// lookup.
 template <class T, bool WIDE_TABLE, int D>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
-  constexpr int kThreads = D / 16;      // threads per head
-  const int heads = a.q_heads + 2 * a.c.kv_heads;
-  const int64_t item = (int64_t(blockIdx.x) * blockDim.x + threadIdx.x) / kThreads;
-  const int lane = threadIdx.x % kThreads;
-  if (item >= int64_t(a.tokens) * heads) return;   // whole groups of kThreads threads leave
-  const int row = int(item / heads), head = int(item % heads);
-
-  // the request this row belongs to: the last one whose rows begin at or before it
-  const int n = a.c.num_requests;
-  int lo = 0, hi = n;   // number of requests whose rows end at or before `row`
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (a.c.qo[mid + 1] <= row) lo = mid + 1;
-    else hi = mid;
-  }
-  if (lo >= n) return;                       // a padding row behind the last request
-  const int req = lo;
-  const PagedRun run = paged_run(a.c.indptr[req], a.c.indptr[req + 1], a.c.last[req], a.c.page_size,
-                                 a.c.num_indices);
-  const int64_t pos = paged_new_position(run, a.c.qo[req + 1], row);
-  if (a.c.qo[req] > row || run.broken || pos < 0 || pos >= run.tokens) {
-    paged_flag(a.c, run.broken ? kPagedBadTable : kPagedBadLength);
-    return;
-  }
-  const bool rotate = a.cos != nullptr;
-  if (rotate && pos >= a.max_pos) {
-    paged_flag(a.c, kPagedBadPosition);
-    return;
-  }
-  const int64_t slot = paged_row(a.c.indices[run.first + pos / a.c.page_size], a.c.num_pages, pos,
-                                 a.c.page_size, a.c.stride_page, a.c.stride_token);
-  if (slot < 0) {
-    paged_flag(a.c, kPagedBadPage);
-    return;
-  }
-
-  const bool is_q = head < a.q_heads;
-  const int kv = is_q ? 0 : (head - a.q_heads) % a.c.kv_heads;
-  const bool is_v = !is_q && head - a.q_heads >= a.c.kv_heads;
-  const char *src;
-  char *dst;
-  if (is_q) {
-    const int g = head / a.group, i = head % a.group;
-    src = a.q + 2 * (row * a.q_token + g * a.q_group + i * a.q_head);
-    dst = a.q_out + 2 * (row * a.o_token + g * a.o_group + i * a.o_head);
-  } else {
-    src = is_v ? a.v + 2 * (row * a.v_token + kv * a.v_head) : a.k + 2 * (row * a.k_token + kv * a.k_head);
-    dst = (is_v ? a.c.v : a.c.k) + 2 * (slot + kv * a.c.stride_head);
-  }
-  const int pairs = a.rot / 16;                  // threads that hold a rotated pair
-  const bool turned = rotate && !is_v && lane < pairs;
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int kLanes = D / 16;                       // threads per head
+  constexpr int kItems = kAppendThreads / kLanes;      // (token, head)s at a time
+  constexpr int kAhead = 4;
+  __shared__ Place s_place[kMaxRows];
+  const int row0 = blockIdx.x * a.rows_per_cta;
+  const int rows = min(a.rows_per_cta, a.tokens - row0);
+  const int heads = min(a.heads_per_cta, a.q_heads + 2 * a.c.kv_heads - int(blockIdx.y) * a.heads_per_cta);
+  const int head0 = blockIdx.y * a.heads_per_cta, count = rows * heads;
+  const int lane = threadIdx.x % kLanes;
+  const int pairs = a.rot / 16;                        // threads that hold a rotated pair
   const int c0 = lane < pairs ? lane : a.rot / 8 + 2 * (lane - pairs);
   const int c1 = lane < pairs ? lane + pairs : c0 + 1;
-  uint4 x0 = *reinterpret_cast<const uint4 *>(src + 16 * c0);
-  uint4 x1 = *reinterpret_cast<const uint4 *>(src + 16 * c1);
-  const char *weight = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
-  if (weight || turned) {
-    float u[8], w[8];
-    op_widen8<T>(x0, u);
-    op_widen8<T>(x1, w);
-    if (weight) {
-      float ss = 0.f;
+  const unsigned group_mask = (kLanes == 32 ? ~0u : (1u << kLanes) - 1u) << (threadIdx.x % 32 / kLanes * kLanes);
+
+  bool placed = false;
+  for (int base = threadIdx.x / kLanes; !placed || base < count; base += kItems * kAhead) {
+    uint4 x0[kAhead], x1[kAhead];
+    int row[kAhead], head[kAhead];       // of the CTA's; head counts q heads, then k, then v
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += u[i] * u[i] + w[i] * w[i];
-      const unsigned mask = ((kThreads == 32 ? 0u : (1u << kThreads)) - 1u) << (threadIdx.x % 32 / kThreads * kThreads);
-#pragma unroll
-      for (int o = kThreads / 2; o; o /= 2) ss += __shfl_xor_sync(mask, ss, o);
-      const float f = rsqrtf(ss * (1.0f / D) + a.eps);
-      float g[8];
-      op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c0)), g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] *= f * g[i];
-      op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c1)), g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] *= f * g[i];
-    }
-    if (turned) {
-      float c[8], s[8], c2[8], s2[8];
-      const int64_t at = pos * a.table_stride;
-      load_table<T, WIDE_TABLE>(a.cos, at + 8 * c0, c);
-      load_table<T, WIDE_TABLE>(a.sin, at + 8 * c0, s);
-      load_table<T, WIDE_TABLE>(a.cos, at + 8 * c1, c2);
-      load_table<T, WIDE_TABLE>(a.sin, at + 8 * c1, s2);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // products and sums rounded one by one, as the attention task of the graph does: K rows
-        // appended by either are the same bits
-        const float y0 = __fadd_rn(__fmul_rn(u[i], c[i]), -__fmul_rn(w[i], s[i]));
-        const float y1 = __fadd_rn(__fmul_rn(w[i], c2[i]), __fmul_rn(u[i], s2[i]));
-        u[i] = y0;
-        w[i] = y1;
+    for (int j = 0; j < kAhead; ++j) {
+      const int item = base + j * kItems;
+      row[j] = item < count ? int(fast_div(item, a.heads_div)) : -1;
+      head[j] = head0 + item - row[j] * heads;
+      if (row[j] < 0) continue;
+      const int64_t r = row0 + row[j];
+      const char *src;
+      if (head[j] < a.q_heads) {
+        const int g = fast_div(head[j], a.group_div);
+        src = a.q + 2 * (r * a.q_token + g * a.q_group + (head[j] - g * a.group) * a.q_head);
+      } else {
+        const int kv = head[j] - a.q_heads;
+        src = kv < a.c.kv_heads ? a.k + 2 * (r * a.k_token + kv * a.k_head)
+                                : a.v + 2 * (r * a.v_token + (kv - a.c.kv_heads) * a.v_head);
       }
+      x0[j] = __ldcs(reinterpret_cast<const uint4 *>(src + 16 * c0));
+      x1[j] = __ldcs(reinterpret_cast<const uint4 *>(src + 16 * c1));
     }
-    x0 = op_round8<T>(u);
-    x1 = op_round8<T>(w);
+    if (!placed) {
+      for (int i = threadIdx.x / 32; i < rows; i += kAppendThreads / 32) {
+        const Place p = find_place(a, row0 + i);
+        if (threadIdx.x % 32 == 0) s_place[i] = p;
+      }
+      __syncthreads();
+      placed = true;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (row[j] < 0) continue;          // (whole groups of kLanes threads together)
+      const Place place = s_place[row[j]];
+      if (place.slot < 0) continue;
+      const int kv = head[j] - a.q_heads;
+      const bool is_q = kv < 0, is_v = kv >= a.c.kv_heads;
+      const char *weight = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
+      const bool turned = a.cos && !is_v && lane < pairs;
+      if (weight || turned) {
+        float u[8], w[8];
+        op_widen8<T>(x0[j], u);
+        op_widen8<T>(x1[j], w);
+        if (weight) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss += u[i] * u[i] + w[i] * w[i];
+#pragma unroll
+          for (int o = kLanes / 2; o; o /= 2) ss += __shfl_xor_sync(group_mask, ss, o);
+          const float f = rsqrtf(ss * (1.0f / D) + a.eps);
+          float g[8];
+          op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c0)), g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[i] *= f * g[i];
+          op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c1)), g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] *= f * g[i];
+        }
+        if (turned) {
+          float c[8], s[8];
+          // products and sums rounded one by one, as the attention task of the graph does: K rows
+          // appended by either are the same bits
+          load_table<T, WIDE_TABLE>(a.cos, place.table + 8 * c0, c);
+          load_table<T, WIDE_TABLE>(a.sin, place.table + 8 * c0, s);
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y[i] = __fadd_rn(__fmul_rn(u[i], c[i]), -__fmul_rn(w[i], s[i]));
+          load_table<T, WIDE_TABLE>(a.cos, place.table + 8 * c1, c);
+          load_table<T, WIDE_TABLE>(a.sin, place.table + 8 * c1, s);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) w[i] = __fadd_rn(__fmul_rn(w[i], c[i]), __fmul_rn(u[i], s[i]));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[i] = y[i];
+        }
+        x0[j] = op_round8<T>(u);
+        x1[j] = op_round8<T>(w);
+      }
+      char *dst;
+      if (is_q) {
+        const int64_t r = row0 + row[j];
+        const int g = fast_div(head[j], a.group_div);
+        dst = a.q_out + 2 * (r * a.o_token + g * a.o_group + (head[j] - g * a.group) * a.o_head);
+      } else {
+        dst = is_v ? a.c.v + 2 * (place.slot + (kv - a.c.kv_heads) * a.c.stride_head)
+                   : a.c.k + 2 * (place.slot + kv * a.c.stride_head);
+      }
+      *reinterpret_cast<uint4 *>(dst + 16 * c0) = x0[j];
+      *reinterpret_cast<uint4 *>(dst + 16 * c1) = x1[j];
+    }
   }
-  *reinterpret_cast<uint4 *>(dst + 16 * c0) = x0;
-  *reinterpret_cast<uint4 *>(dst + 16 * c1) = x1;
+}
+
+// A few calls' tokens fill no device: then a CTA takes one token's share of the heads, so that
+// every thread has one (token, head) to move; many tokens: whole tokens, eight to a CTA, whose
+// lookups and table rows serve all heads.
+template <class T, bool WIDE_TABLE, int D>
+int launch_shape(AppendArgs &a, cudaStream_t st) {
+  const int heads = a.q_heads + 2 * a.c.kv_heads, at_once = kAppendThreads / (D / 16);
+  const bool few = int64_t(a.tokens) * heads <= int64_t(at_once) * 148 * 8;
+  a.rows_per_cta = few ? 1 : kMaxRows;
+  a.heads_per_cta = few ? std::min(heads, at_once) : heads;
+  a.heads_div = fast_divisor(a.heads_per_cta);
+  a.group_div = fast_divisor(a.group);
+  const dim3 grid((a.tokens + a.rows_per_cta - 1) / a.rows_per_cta, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
+  if (grid.y > 65535) return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d heads", heads);
+  paged_append_kernel<T, WIDE_TABLE, D><<<grid, kAppendThreads, 0, st>>>(a);
+  return op_launched("paged_append");
 }
 
 template <class T, bool WIDE_TABLE>
-int launch_append(int head_dim, const AppendArgs &a, cudaStream_t st) {
-  const int64_t items = int64_t(a.tokens) * (a.q_heads + 2 * a.c.kv_heads);
-  const int64_t threads = items * (head_dim / 16);
-  const int64_t blocks = (threads + 255) / 256;
-  if (blocks > 0x7fffffff) return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d tokens in one call", a.tokens);
-  if (head_dim == 64) paged_append_kernel<T, WIDE_TABLE, 64><<<unsigned(blocks), 256, 0, st>>>(a);
-  else if (head_dim == 128) paged_append_kernel<T, WIDE_TABLE, 128><<<unsigned(blocks), 256, 0, st>>>(a);
-  else paged_append_kernel<T, WIDE_TABLE, 256><<<unsigned(blocks), 256, 0, st>>>(a);
-  return op_launched("paged_append");
+int launch_append(int head_dim, AppendArgs &a, cudaStream_t st) {
+  if (head_dim == 64) return launch_shape<T, WIDE_TABLE, 64>(a, st);
+  if (head_dim == 128) return launch_shape<T, WIDE_TABLE, 128>(a, st);
+  return launch_shape<T, WIDE_TABLE, 256>(a, st);
 }
 
 bool strides_ok(std::initializer_list<int64_t> s) {
