@@ -26,7 +26,35 @@ struct OpF16 {
   }
 };
 
-// Eight elements of 16 bits (one 16-byte load) as floats, and back.
+// Pairs of fp32 in one 64-bit register: one instruction for both, each rounded as usual.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Eight elements of 16 bits (one 16-byte load) as floats or pairs, and back.
 template <class T>
 __device__ __forceinline__ void op_widen8(const uint4 &v, float (&x)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -39,8 +67,19 @@ __device__ __forceinline__ void op_widen8(const uint4 &v, float (&x)[8]) {
 }
 
 template <class T>
-__device__ __forceinline__ uint4 op_round8(const float (&x)[8]) {
-  return make_uint4(T::round2(x[0], x[1]), T::round2(x[2], x[3]), T::round2(x[4], x[5]), T::round2(x[6], x[7]));
+__device__ __forceinline__ void op_widen8(const uint4 &v, f32x2 (&x)[4]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = T::widen(w[i]);
+    x[i] = pair(f.x, f.y);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ uint4 op_round8(const f32x2 (&x)[4]) {
+  const float2 a = halves(x[0]), b = halves(x[1]), c = halves(x[2]), d = halves(x[3]);
+  return make_uint4(T::round2(a.x, a.y), T::round2(b.x, b.y), T::round2(c.x, c.y), T::round2(d.x, d.y));
 }
 
 }  // namespace ypk

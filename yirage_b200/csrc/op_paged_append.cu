@@ -66,20 +66,20 @@ struct AppendArgs {
   int64_t table_stride;
   int tokens, q_heads, group, rot, max_pos;
   int rows_per_cta, heads_per_cta;
-  FastDivisor heads_div, group_div;
   float eps;
 };
 
 constexpr int kAppendThreads = 128;
 constexpr int kMaxRows = 8;          // tokens per CTA
+constexpr int kAhead = 3;            // heads per thread
 
-// Eight table values as floats, from 16 or 32 bits.
+// Eight table values as pairs of floats, from 16 or 32 bits.
 template <class T, bool WIDE_TABLE>
-__device__ __forceinline__ void load_table(const char *base, int64_t element, float (&x)[8]) {
+__device__ __forceinline__ void load_table(const char *base, int64_t element, f32x2 (&x)[4]) {
   if (WIDE_TABLE) {
     const float4 *p = reinterpret_cast<const float4 *>(base + element * 4);
     const float4 a = __ldg(p), b = __ldg(p + 1);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    x[0] = pair(a.x, a.y), x[1] = pair(a.z, a.w), x[2] = pair(b.x, b.y), x[3] = pair(b.z, b.w);
   } else {
     op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(base + element * 2)), x);
   }
@@ -91,17 +91,19 @@ struct Place {
   int64_t table;   // element offset of its row in the rotary tables
 };
 
-// The place of row `row`, found by a whole warp.  Broken entries are reported and give slot -1.
+// The places of the rows of a warp's groups of LANES threads, one row per group; all lanes call.
+// Broken entries are reported and give slot -1.
+template <int LANES>
 __device__ __forceinline__ Place find_place(const AppendArgs &a, int row) {
-  const int lane = threadIdx.x % 32;
-  // the request whose rows hold this one: rounds of 32 evenly spaced looks at the row offsets
+  const int lane = threadIdx.x % LANES, shift = threadIdx.x % 32 / LANES * LANES;
+  // the request whose rows hold this one: rounds of LANES evenly spaced looks at the row offsets
   int lo = 0, n = a.c.num_requests;      // the answer is among requests lo .. lo + n
-  while (n > 0) {
-    const int step = (n + 31) / 32, at = lo + (lane + 1) * step;     // requests lo .. at - 1 end before?
-    const bool before = at <= lo + n && __ldg(a.c.qo + at) <= row;
-    const int skip = __popc(__ballot_sync(~0u, before)) * step;
+  while (__any_sync(~0u, n > 0)) {
+    const int step = (n + LANES - 1) / LANES, at = lo + (lane + 1) * step;
+    const bool before = n > 0 && at <= lo + n && __ldg(a.c.qo + at) <= row;   // requests lo .. at - 1 end before
+    const int skip = __popc(__ballot_sync(~0u, before) >> shift & ((1u << LANES) - 1)) * step;
     lo += skip;
-    n = min(n - skip, step - 1);
+    n = n > 0 ? min(n - skip, step - 1) : 0;
   }
   Place p = {-1, 0};
   if (lo >= a.c.num_requests) return p;                              // a padding row
@@ -122,131 +124,146 @@ __device__ __forceinline__ Place find_place(const AppendArgs &a, int row) {
   return p;
 }
 
-// A CTA takes a.rows_per_cta tokens and, of each, the heads of blockIdx.y's share.  Its warps look
-// up where the tokens go; then D / 16 threads move one (token, head), each two chunks of eight
-// dimensions: the pair that a rotation mixes, or two neighbours behind the rotated part.  Four
-// (token, head)s per thread are read before the first is finished, the first four before the
-// lookup.
+// A CTA takes a.rows_per_cta tokens and, of each, the heads of blockIdx.y's share (q heads, then k,
+// then v).  D / 16 threads move one head at a time, each thread two chunks of eight dimensions:
+// the pair that a rotation mixes, or two neighbours behind the rotated part.  A thread keeps its
+// kAhead heads from token to token, so what belongs to a head (addresses, kind, norm weight)
+// is worked out once, and a token's table entries serve all of them; the next token's rows are
+// on their way while one is finished, the first ones while the places are looked up.
 template <class T, bool WIDE_TABLE, int D>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads, 4) paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int kLanes = D / 16;                       // threads per head
-  constexpr int kItems = kAppendThreads / kLanes;      // (token, head)s at a time
-  constexpr int kAhead = 4;
+  constexpr int kItems = kAppendThreads / kLanes;      // heads at a time
   __shared__ Place s_place[kMaxRows];
-  const int row0 = blockIdx.x * a.rows_per_cta;
-  const int rows = min(a.rows_per_cta, a.tokens - row0);
-  const int heads = min(a.heads_per_cta, a.q_heads + 2 * a.c.kv_heads - int(blockIdx.y) * a.heads_per_cta);
-  const int head0 = blockIdx.y * a.heads_per_cta, count = rows * heads;
+  const int64_t row0 = int64_t(blockIdx.x) * a.rows_per_cta;
+  const int rows = int(min(int64_t(a.rows_per_cta), a.tokens - row0));
   const int lane = threadIdx.x % kLanes;
   const int pairs = a.rot / 16;                        // threads that hold a rotated pair
   const int c0 = lane < pairs ? lane : a.rot / 8 + 2 * (lane - pairs);
   const int c1 = lane < pairs ? lane + pairs : c0 + 1;
-  const unsigned group_mask = (kLanes == 32 ? ~0u : (1u << kLanes) - 1u) << (threadIdx.x % 32 / kLanes * kLanes);
+  const unsigned group_mask = ((1u << kLanes) - 1u) << (threadIdx.x % 32 / kLanes * kLanes);
+  const bool turns = a.cos && lane < pairs;
 
-  bool placed = false;
-  for (int base = threadIdx.x / kLanes; !placed || base < count; base += kItems * kAhead) {
+  // this thread's heads
+  const char *src[kAhead];
+  char *dst[kAhead];
+  int64_t src_step[kAhead];
+  int kind[kAhead];                                    // 0: q, 1: k, 2: v, -1: none
+  const int heads = a.q_heads + 2 * a.c.kv_heads;
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) {
+    const int in_share = threadIdx.x / kLanes + j * kItems, h = blockIdx.y * a.heads_per_cta + in_share;
+    kind[j] = in_share >= a.heads_per_cta || h >= heads ? -1 : h < a.q_heads ? 0 : h < a.q_heads + a.c.kv_heads ? 1 : 2;
+    const int kv = (h - a.q_heads) - (kind[j] == 2 ? a.c.kv_heads : 0);
+    if (kind[j] == 0) {
+      const int g = h / a.group, i = h - g * a.group;
+      src_step[j] = a.q_token;
+      src[j] = a.q + 2 * (g * a.q_group + i * a.q_head);
+      dst[j] = a.q_out + 2 * (row0 * a.o_token + g * a.o_group + i * a.o_head);
+    } else if (kind[j] == 1) {
+      src_step[j] = a.k_token;
+      src[j] = a.k + 2 * (kv * a.k_head);
+      dst[j] = a.c.k + 2 * (kv * a.c.stride_head);
+    } else {
+      src_step[j] = a.v_token;
+      src[j] = a.v + 2 * (kv * a.v_head);
+      dst[j] = a.c.v + 2 * (kv * a.c.stride_head);
+    }
+    src[j] += 2 * row0 * src_step[j];
+    src_step[j] *= 2;
+  }
+  uint4 n0[kAhead], n1[kAhead];
+  const auto fetch = [&]() {       // the rows at src, which moves on
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (kind[j] >= 0) {
+        n0[j] = __ldcs(reinterpret_cast<const uint4 *>(src[j] + 16 * c0));
+        n1[j] = __ldcs(reinterpret_cast<const uint4 *>(src[j] + 16 * c1));
+      }
+      src[j] += src_step[j];
+    }
+  };
+  fetch();
+  {
+    static_assert(kItems >= kMaxRows, "one group of threads looks up one token");
+    const int i = threadIdx.x / kLanes;
+    if (threadIdx.x / 32 * 32 / kLanes < rows) {       // (whole warps)
+      const Place p = find_place<kLanes>(a, int(row0) + min(i, rows - 1));
+      if (lane == 0 && i < rows) s_place[i] = p;
+    }
+  }
+  __syncthreads();
+
+  for (int t = 0; t < rows; ++t) {
     uint4 x0[kAhead], x1[kAhead];
-    int row[kAhead], head[kAhead];       // of the CTA's; head counts q heads, then k, then v
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const int item = base + j * kItems;
-      row[j] = item < count ? int(fast_div(item, a.heads_div)) : -1;
-      head[j] = head0 + item - row[j] * heads;
-      if (row[j] < 0) continue;
-      const int64_t r = row0 + row[j];
-      const char *src;
-      if (head[j] < a.q_heads) {
-        const int g = fast_div(head[j], a.group_div);
-        src = a.q + 2 * (r * a.q_token + g * a.q_group + (head[j] - g * a.group) * a.q_head);
-      } else {
-        const int kv = head[j] - a.q_heads;
-        src = kv < a.c.kv_heads ? a.k + 2 * (r * a.k_token + kv * a.k_head)
-                                : a.v + 2 * (r * a.v_token + (kv - a.c.kv_heads) * a.v_head);
-      }
-      x0[j] = __ldcs(reinterpret_cast<const uint4 *>(src + 16 * c0));
-      x1[j] = __ldcs(reinterpret_cast<const uint4 *>(src + 16 * c1));
-    }
-    if (!placed) {
-      for (int i = threadIdx.x / 32; i < rows; i += kAppendThreads / 32) {
-        const Place p = find_place(a, row0 + i);
-        if (threadIdx.x % 32 == 0) s_place[i] = p;
-      }
-      __syncthreads();
-      placed = true;
+    for (int j = 0; j < kAhead; ++j) x0[j] = n0[j], x1[j] = n1[j];
+    if (t + 1 < rows) fetch();
+    const Place place = s_place[t];
+    if (place.slot < 0) continue;
+    f32x2 cos0[4], sin0[4], cos1[4], sin1[4];         // sin0: negated
+    if (turns) {
+      load_table<T, WIDE_TABLE>(a.cos, place.table + 8 * c0, cos0);
+      load_table<T, WIDE_TABLE>(a.sin, place.table + 8 * c0, sin0);
+      load_table<T, WIDE_TABLE>(a.cos, place.table + 8 * c1, cos1);
+      load_table<T, WIDE_TABLE>(a.sin, place.table + 8 * c1, sin1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sin0[i] ^= 0x8000000080000000ull;
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (row[j] < 0) continue;          // (whole groups of kLanes threads together)
-      const Place place = s_place[row[j]];
-      if (place.slot < 0) continue;
-      const int kv = head[j] - a.q_heads;
-      const bool is_q = kv < 0, is_v = kv >= a.c.kv_heads;
-      const char *weight = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
-      const bool turned = a.cos && !is_v && lane < pairs;
-      if (weight || turned) {
-        float u[8], w[8];
+      if (kind[j] < 0) continue;          // (whole groups of kLanes threads together)
+      const char *weight = kind[j] == 0 ? a.q_norm : kind[j] == 1 ? a.k_norm : nullptr;
+      if (weight || (turns && kind[j] < 2)) {
+        f32x2 u[4], w[4];
         op_widen8<T>(x0[j], u);
         op_widen8<T>(x1[j], w);
         if (weight) {
-          float ss = 0.f;
+          f32x2 ss = 0;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss += u[i] * u[i] + w[i] * w[i];
+          for (int i = 0; i < 4; ++i) ss = fma2(u[i], u[i], fma2(w[i], w[i], ss));
+          const float2 s2 = halves(ss);
+          float total = s2.x + s2.y;
 #pragma unroll
-          for (int o = kLanes / 2; o; o /= 2) ss += __shfl_xor_sync(group_mask, ss, o);
-          const float f = rsqrtf(ss * (1.0f / D) + a.eps);
-          float g[8];
+          for (int o = kLanes / 2; o; o /= 2) total += __shfl_xor_sync(group_mask, total, o);
+          const float f = rsqrtf(total * (1.0f / D) + a.eps);
+          f32x2 g[4];
           op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c0)), g);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) u[i] *= f * g[i];
+          for (int i = 0; i < 4; ++i) u[i] = mul2(mul2(u[i], pair(f, f)), g[i]);
           op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c1)), g);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] *= f * g[i];
+          for (int i = 0; i < 4; ++i) w[i] = mul2(mul2(w[i], pair(f, f)), g[i]);
         }
-        if (turned) {
-          float c[8], s[8];
+        if (turns) {
           // products and sums rounded one by one, as the attention task of the graph does: K rows
           // appended by either are the same bits
-          load_table<T, WIDE_TABLE>(a.cos, place.table + 8 * c0, c);
-          load_table<T, WIDE_TABLE>(a.sin, place.table + 8 * c0, s);
-          float y[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = __fadd_rn(__fmul_rn(u[i], c[i]), -__fmul_rn(w[i], s[i]));
-          load_table<T, WIDE_TABLE>(a.cos, place.table + 8 * c1, c);
-          load_table<T, WIDE_TABLE>(a.sin, place.table + 8 * c1, s);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = __fadd_rn(__fmul_rn(w[i], c[i]), __fmul_rn(u[i], s[i]));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) u[i] = y[i];
+          for (int i = 0; i < 4; ++i) {
+            const f32x2 y = add2(mul2(u[i], cos0[i]), mul2(w[i], sin0[i]));
+            w[i] = add2(mul2(w[i], cos1[i]), mul2(u[i], sin1[i]));
+            u[i] = y;
+          }
         }
         x0[j] = op_round8<T>(u);
         x1[j] = op_round8<T>(w);
       }
-      char *dst;
-      if (is_q) {
-        const int64_t r = row0 + row[j];
-        const int g = fast_div(head[j], a.group_div);
-        dst = a.q_out + 2 * (r * a.o_token + g * a.o_group + (head[j] - g * a.group) * a.o_head);
-      } else {
-        dst = is_v ? a.c.v + 2 * (place.slot + (kv - a.c.kv_heads) * a.c.stride_head)
-                   : a.c.k + 2 * (place.slot + kv * a.c.stride_head);
-      }
-      *reinterpret_cast<uint4 *>(dst + 16 * c0) = x0[j];
-      *reinterpret_cast<uint4 *>(dst + 16 * c1) = x1[j];
+      char *to = dst[j] + (kind[j] == 0 ? 2 * t * a.o_token : 2 * place.slot);
+      *reinterpret_cast<uint4 *>(to + 16 * c0) = x0[j];
+      *reinterpret_cast<uint4 *>(to + 16 * c1) = x1[j];
     }
   }
 }
 
-// A few calls' tokens fill no device: then a CTA takes one token's share of the heads, so that
-// every thread has one (token, head) to move; many tokens: whole tokens, eight to a CTA, whose
-// lookups and table rows serve all heads.
+// Few tokens: a CTA takes one token and as many of its heads as it moves at a time, so that one
+// token's heads spread over the device.  Many: kMaxRows tokens, kAhead times as many heads.
 template <class T, bool WIDE_TABLE, int D>
 int launch_shape(AppendArgs &a, cudaStream_t st) {
-  const int heads = a.q_heads + 2 * a.c.kv_heads, at_once = kAppendThreads / (D / 16);
-  const bool few = int64_t(a.tokens) * heads <= int64_t(at_once) * 148 * 8;
+  constexpr int kItems = kAppendThreads / (D / 16);
+  const int heads = a.q_heads + 2 * a.c.kv_heads;
+  const bool few = int64_t(a.tokens) * heads <= int64_t(kItems) * 148 * 8;
   a.rows_per_cta = few ? 1 : kMaxRows;
-  a.heads_per_cta = few ? std::min(heads, at_once) : heads;
-  a.heads_div = fast_divisor(a.heads_per_cta);
-  a.group_div = fast_divisor(a.group);
+  a.heads_per_cta = few ? kItems : kItems * kAhead;
   const dim3 grid((a.tokens + a.rows_per_cta - 1) / a.rows_per_cta, (heads + a.heads_per_cta - 1) / a.heads_per_cta);
   if (grid.y > 65535) return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d heads", heads);
   paged_append_kernel<T, WIDE_TABLE, D><<<grid, kAppendThreads, 0, st>>>(a);
