@@ -109,6 +109,12 @@ struct Vec<YPK_F32> {
   static __device__ __forceinline__ float top(const uint4 &v) {
     return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
+  static __device__ __forceinline__ uint4 larger(const uint4 &a, const uint4 &b) {      // element by element
+    return make_uint4(larger1(a.x, b.x), larger1(a.y, b.y), larger1(a.z, b.z), larger1(a.w, b.w));
+  }
+  static __device__ __forceinline__ uint32_t larger1(uint32_t a, uint32_t b) {
+    return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+  }
   static __device__ __forceinline__ float2 two(const uint4 &v, int i) {
     return i ? make_float2(__uint_as_float(v.z), __uint_as_float(v.w)) : make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
   }
@@ -135,6 +141,9 @@ struct Vec<YPK_BF16> {
   static __device__ __forceinline__ float top(const uint4 &v) {
     const float2 f = OpBf16::widen(max2(max2(v.x, v.y), max2(v.z, v.w)));
     return max_nan(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint4 larger(const uint4 &a, const uint4 &b) {
+    return make_uint4(max2(a.x, b.x), max2(a.y, b.y), max2(a.z, b.z), max2(a.w, b.w));
   }
   static __device__ __forceinline__ float2 two(const uint4 &v, int i) {
     return OpBf16::widen(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
@@ -164,6 +173,9 @@ struct Vec<YPK_F16> {
   static __device__ __forceinline__ float top(const uint4 &v) {
     const float2 f = OpF16::widen(max2(max2(v.x, v.y), max2(v.z, v.w)));
     return max_nan(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint4 larger(const uint4 &a, const uint4 &b) {
+    return make_uint4(max2(a.x, b.x), max2(a.y, b.y), max2(a.z, b.z), max2(a.w, b.w));
   }
   static __device__ __forceinline__ float2 two(const uint4 &v, int i) {
     return OpF16::widen(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
@@ -420,9 +432,10 @@ struct Running {
 
   template <int N>
   __device__ __forceinline__ float take(const uint4 (&x)[N]) {      // the largest of x
-    float t = V::top(x[0]);
+    uint4 most = x[0];
 #pragma unroll
-    for (int j = 1; j < N; ++j) t = max_nan(t, V::top(x[j]));
+    for (int j = 1; j < N; ++j) most = V::larger(most, x[j]);
+    const float t = V::top(most);
     top = max_nan(top, t);
     if (!(t >= V::kLow)) return t;      // nothing here that counts beside a higher value
     if (t > m) {
