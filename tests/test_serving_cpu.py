@@ -221,11 +221,18 @@ int main() {
     }
   }
   // rows: inside the pool, at 64-bit offsets, or refused
-  for (int page : offsets) for (int pages : {1, 8, big}) for (int ps : {1, 3, 16, 64}) for (int64_t pos : {0L, 1L, 15L, 16L, 1000L, 1L << 40}) {
-    const int64_t st = 1024, sp = st * ps, row = paged_row(page, pages, pos, ps, sp, st);
+  for (int page : offsets) for (int pages : {1, 8, big}) for (int ps : {1, 3, 16, 64, 4096}) for (int pos : {0, 1, 15, 16, 1000, big - 255}) {
+    const int q = fast_div(pos, fast_divisor(ps)), in = pos - q * ps;
+    need(q == pos / ps && in == pos % ps, "page of a position");
+    const int64_t st = 1024, sp = st * ps, row = paged_row(page, pages, in, sp, st);
     if (page < 0 || page >= pages) need(row == -1, "page outside the pool");
-    else need(row == page * sp + (pos % ps) * st && row >= 0 && row + st <= int64_t(pages) * sp, "row");
+    else need(row == page * sp + in * st && row >= 0 && row + st <= int64_t(pages) * sp, "row");
   }
+  // division without one: every divisor up to 5000 and some large ones, at and around its multiples
+  for (int64_t d = 1; d <= big; d = d < 5000 ? d + 1 : d * 3 + 1)
+    for (int64_t m : {int64_t(0), int64_t(1), int64_t(2), int64_t(77), big / d - 1, big / d})
+      for (int64_t n = m * d - 1; n <= m * d + 1; ++n)
+        if (n >= 0 && n <= big) need(fast_div(int(n), fast_divisor(int(d))) == n / d, "fast_div");
   std::puts("ok");
 }
 """

@@ -67,6 +67,7 @@ struct AppendArgs {
   int tokens, q_heads, group, rot, max_pos;
   int rows_per_cta, rows_at_once;   // tokens a CTA takes; as many of them together
   int heads_per_cta;
+  FastDivisor page_div;
   float eps;
 };
 
@@ -118,8 +119,8 @@ __device__ __forceinline__ Place find_place(const AppendArgs &a, int row) {
   else if (__ldg(a.c.qo + lo) > row || pos < 0 || pos >= run.tokens) bad = kPagedBadLength;
   else if (a.cos && pos >= a.max_pos) bad = kPagedBadPosition;
   else {
-    const int page = __ldg(a.c.indices + run.first + int(pos) / a.c.page_size);
-    p.slot = paged_row(page, a.c.num_pages, pos, a.c.page_size, a.c.stride_page, a.c.stride_token);
+    const int q = fast_div(int(pos), a.page_div), page = __ldg(a.c.indices + run.first + q);
+    p.slot = paged_row(page, a.c.num_pages, int(pos) - q * a.c.page_size, a.c.stride_page, a.c.stride_token);
     p.table = pos * a.table_stride;
     if (p.slot < 0) bad = kPagedBadPage;
   }
@@ -356,6 +357,7 @@ extern "C" int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_ap
   a.rot = p->cos ? p->rot_dim : 0;
   a.max_pos = p->max_positions;
   a.eps = p->eps;
+  a.page_div = fast_divisor(cache->page_size);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (cache->dtype == YPK_BF16)
     return wide ? launch_append<OpBf16, true>(cache->head_dim, a, st) : launch_append<OpBf16, false>(cache->head_dim, a, st);

@@ -43,6 +43,7 @@ struct DecodeArgs {
   int ctas;            // per (request, pass) where clusters are used
   int head_blocks;     // passes over a K/V head's rows: ceil(group / (8 NT))
   int heads_per_pass;  // query heads of one pass, at most 8 NT
+  FastDivisor page_div;
   float scale_log2;
   // workspace
   int by_segment;      // the segments are few: desc is indexed by segment, not by worker
@@ -307,8 +308,10 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   const uint32_t my_ring32 = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
   Segment fs = begin;
   int fj = fs.ja + warp;
-  int page = 0;                // of this lane's row (lane % 16) in the block at the cursor
+  int page = 0, in_page = 0;   // of this lane's row (lane % 16) in the block at the cursor; -1: not seen
+  int64_t head_at = 0;         // element offset of the segment's K/V head
   bool more = true;            // the cursor stands on a block
+  const auto enter = [&]() { head_at = fs.pass / a.head_blocks * a.c.stride_head; };
   const auto settle = [&]() {  // move the cursor onto a block, fetch its page numbers
     while (fj >= fs.jb) {
       if (fs.left == 0) {
@@ -317,20 +320,21 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       }
       next_segment(fs);
       fj = warp;
+      enter();
     }
     const int pos = (fs.b0 + fj) * kBlock + lane % kBlock;
-    page = pos < fs.len && pos >= fs.lo ? __ldg(a.c.indices + fs.first + pos / a.c.page_size) : -1;
+    const int q = fast_div(pos, a.page_div);
+    in_page = pos < fs.len && pos >= fs.lo ? pos - q * a.c.page_size : -1;
+    page = in_page >= 0 ? __ldg(a.c.indices + fs.first + q) : -1;
   };
   int fstage = 0;
   const auto issue = [&]() {
     if (more) {
-      const int pos = (fs.b0 + fj) * kBlock + lane % kBlock;
-      const bool inside = pos < fs.len && pos >= fs.lo;
-      int64_t row = inside ? paged_row(page, a.c.num_pages, pos, a.c.page_size, a.c.stride_page, a.c.stride_token) : -1;
-      if (inside && row < 0) paged_flag(a.c, kPagedBadPage);
+      int64_t row = in_page >= 0 ? paged_row(page, a.c.num_pages, in_page, a.c.stride_page, a.c.stride_token) : -1;
+      if (in_page >= 0 && row < 0) paged_flag(a.c, kPagedBadPage);
       const unsigned mask = __ballot_sync(~0u, row >= 0) & 0xffffu;
       if (lane == 0) s_mask[warp * S + fstage] = int(mask);
-      if (row >= 0) row = 2 * (row + (fs.pass / a.head_blocks) * a.c.stride_head);
+      if (row >= 0) row = 2 * (row + head_at);
       const uint32_t dst = my_ring32 + fstage * 2 * Shape::kTile;
 #pragma unroll
       for (int i = 0; i < kBlock * kChunks / 32; ++i) {
@@ -348,6 +352,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  enter();
   settle();
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) issue();
@@ -802,6 +807,7 @@ extern "C" int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_de
   a.heads_per_pass = pass_heads(cache->head_dim, a.group);
   a.head_blocks = (a.group + a.heads_per_pass - 1) / a.heads_per_pass;
   a.ctas = cluster_ctas(cache, p->rows, cache->num_kv_heads * a.head_blocks, p->window, dev.sms);
+  a.page_div = fast_divisor(cache->page_size);
   a.by_segment = int64_t(p->rows) * cache->num_kv_heads * a.head_blocks <= dev.sms;
   a.scale_log2 = p->scale * 1.4426950408889634f;
   const uint64_t need = workspace_bytes(dev.sms, a.heads_per_pass, cache->head_dim);

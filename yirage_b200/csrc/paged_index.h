@@ -55,12 +55,31 @@ YPK_HD int64_t paged_new_position(const PagedRun &run, int qo_end, int row) {
   return behind < 1 ? -1 : run.tokens - behind;
 }
 
-// Element offset of a position's row for K/V head 0, or -1 when its page is not in the pool.
-// `pos` lies in [0, run.tokens).
-YPK_HD int64_t paged_row(int page, int num_pages, int64_t pos, int page_size, int64_t stride_page,
-                         int64_t stride_token) {
+// Element offset of a row for K/V head 0, or -1 when the page is not in the pool.  `in_page`: its
+// place in the page, in [0, page_size).
+YPK_HD int64_t paged_row(int page, int num_pages, int in_page, int64_t stride_page, int64_t stride_token) {
   if (page < 0 || page >= num_pages) return -1;
-  return int64_t(page) * stride_page + (pos % page_size) * stride_token;
+  return int64_t(page) * stride_page + int64_t(in_page) * stride_token;
+}
+
+// n / d for 0 <= n < 2^31 and 1 <= d < 2^31 without a division: with l = ceil(log2 d) and
+// mul = floor(2^32 (2^l - d) / d) + 1, n / d = (n + mulhi(n, mul)) >> l (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994).
+struct FastDivisor {
+  uint32_t mul, shift;
+};
+inline FastDivisor fast_divisor(int d) {
+  uint32_t l = 0;
+  while ((uint64_t(1) << l) < uint64_t(d)) ++l;
+  return {uint32_t((((uint64_t(1) << l) - uint64_t(d)) << 32) / uint64_t(d) + 1), l};
+}
+YPK_HD int fast_div(int n, const FastDivisor &d) {
+#ifdef __CUDA_ARCH__
+  const uint32_t hi = __umulhi(uint32_t(n), d.mul);
+#else
+  const uint32_t hi = uint32_t((uint64_t(uint32_t(n)) * d.mul) >> 32);
+#endif
+  return int((uint32_t(n) + hi) >> d.shift);
 }
 
 }  // namespace ypk
