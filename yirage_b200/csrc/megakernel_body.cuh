@@ -163,7 +163,9 @@ __device__ __forceinline__ void megakernel_body(const Runtime &rt) {
         __syncwarp();
         wc.task = ti;
         const ypk_task &t = misc->ptask;
-        if (MOE && t.type == YPK_TASK_LINEAR && (t.flags & YPK_F_MOE)) {
+        const bool pick = MOE && t.type == YPK_TASK_LINEAR && (t.flags & YPK_F_MOE);
+        if (MOE) __syncwarp();   // every lane has looked before lane 0 rewrites the task copy
+        if (pick) {
           // the expert whose rows are streamed is known once the router has run
           int go = 1;
           if (lane == 0) go = moe_resolve(wc, rt, &misc->ptask, iter, true);
@@ -209,7 +211,10 @@ __device__ __forceinline__ void megakernel_body(const Runtime &rt) {
           ok = misc->flag != 0;
         }
         if (prec) prec[2] = globaltimer();
-        if (MOE && ok && t.type == YPK_TASK_LINEAR && (t.flags & YPK_F_MOE)) {
+        // Whether the task picks an expert is read from the graph, not from the copy: thread 0 may
+        // turn the copy into a NOP while a slower warp still looks at it, and that warp would
+        // then miss the barrier in here (and the CTA hang in a later one).
+        if (MOE && ok && (t.flags & YPK_F_MOE) && __ldg(&rt.tasks[ti].type) == YPK_TASK_LINEAR) {
           if (tid == 0) moe_resolve(wc, rt, &misc->ctask, iter, false);   // may turn the task into a NOP
           consumer_bar();
         }
