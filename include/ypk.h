@@ -440,7 +440,7 @@ typedef struct ypk_paged_cache {
 typedef struct ypk_paged_append_args {
   const void *k, *v;            /* [num_tokens][num_kv_heads][head_dim]            */
   const void *q;                /* [num_tokens][group..][head_dim], or NULL        */
-  void *q_out;                  /* rotated queries [num_tokens][num_q_heads][head_dim]; may be q */
+  void *q_out;                  /* rotated queries, like q; q itself or apart from it */
   const void *cos, *sin;        /* [max_positions][rot_dim]; NULL: no rotation     */
   const void *q_norm, *k_norm;  /* [head_dim] in the cache's type; NULL: no norm   */
   int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
@@ -461,13 +461,14 @@ typedef struct ypk_paged_append_args {
  * halves: y[i] = x[i] cos[i] - x[i + h] sin[i], y[i + h] = x[i + h] cos[i + h] + x[i] sin[i + h],
  * h = rot_dim / 2, in 32 bits with one rounding at the end.  Rows of k, v and q behind
  * qo_indptr[num_requests] are not read into anything; the rows of q_out there stay as they
- * were, and so do those of dropped tokens. */
+ * were, and so do those of dropped tokens.  Two rows of a call must not go to the same place (two
+ * requests that share a last page). */
 int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_append_args *args, void *stream);
 
 /* Operands of ypk_paged_decode. */
 typedef struct ypk_paged_decode_args {
   const void *q;                /* [rows][group..][head_dim], grouped as in ypk_paged_append */
-  void *out;                    /* [rows][num_q_heads][head_dim]                   */
+  void *out;                    /* like q, apart from it                           */
   float *lse;                   /* [rows][num_q_heads] contiguous, or NULL         */
   void *workspace;              /* ypk_paged_decode_workspace bytes, 16-byte aligned; holds
                                    nothing between calls, not shared by calls that overlap */

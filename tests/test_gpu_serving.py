@@ -184,6 +184,18 @@ def test_decode_nan_in_a_seen_position_shows():
 def test_decode_many_requests():
     lengths = [(37 * i) % 190 for i in range(700)]
     run_decode(lengths, hq=4, heads=1, dim=64, page=16, seed=12)
+    # as many as a call takes: the tables cost the ring a block per warp
+    lengths = [(7 * i) % 50 for i in range(4096)]
+    b = Batch(lengths, heads=1, dim=128, page=16, seed=13)
+    q = rnd(gen(14), 4096, 16, 128)
+    out = b.cache.decode(q)
+    b.cache.check()
+    for r in range(0, 4096, 97):
+        at = b.where(r, torch.arange(lengths[r], device="cuda"))
+        if lengths[r]:
+            check_attention(out[r], None, q[r], b.k[at], b.v[at], 128 ** -0.5, BF16)
+        else:
+            assert (out[r] == 0).all()
 
 
 def test_decode_query_views_outputs_and_rows_behind():
@@ -763,6 +775,59 @@ def test_two_streams_and_two_graphs_at_once():
             g2.replay()
     torch.cuda.synchronize()
     assert same(0, o1) and same(1, o2) and same(2, l1) and same(3, l2)
+
+
+FIRST_CALL = """
+import torch, yirage_b200 as yr
+i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+k = torch.randn(5, 64, 2, 128, device="cuda").bfloat16()
+cache = yr.PagedKVCache(k, k.clone(), {"qo_indptr_buffer": i32([0, 1]), "paged_kv_indptr_buffer": i32([0, 4]),
+                        "paged_kv_indices_buffer": i32([3, 1, 0, 2] * PAGES), "paged_kv_last_page_len_buffer": i32([9])})
+q, n, x, t = (torch.randn(1, 8, 128, device="cuda").bfloat16(), torch.randn(1, 2, 128, device="cuda").bfloat16(),
+              torch.randn(3, 5000, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda"))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    r = cache.append(n, n, q=q)
+    o = cache.decode(r)
+    p = yr.token_logprobs(x, t, top_k=2)
+g.replay()
+torch.cuda.synchronize()
+r2 = cache.append(n, n, q=q)
+assert torch.equal(o, cache.decode(r2)) and torch.equal(p.top_token, yr.token_logprobs(x, t, top_k=2).top_token)
+cache.check()
+print("fine")
+"""
+
+
+@pytest.mark.parametrize("pages", [1, 1000])      # clusters; equal ranges (the page list could be long)
+def test_first_call_of_a_process_may_be_captured(pages):
+    import subprocess
+    import sys
+    out = subprocess.run([sys.executable, "-c", FIRST_CALL.replace("PAGES", str(pages))], capture_output=True, text=True,
+                         timeout=200)
+    assert out.returncode == 0 and out.stdout.strip() == "fine", out.stderr[-2000:]
+
+
+def test_empty_calls_and_shared_memory():
+    b = Batch([30, 20], [1, 1], seed=50)
+    e = torch.empty(0, 2, 128, dtype=BF16, device="cuda")
+    assert b.cache.append(e, e, q=torch.empty(0, 8, 128, dtype=BF16, device="cuda")).shape == (0, 8, 128)
+    out, lse = b.cache.decode(torch.empty(0, 8, 128, dtype=BF16, device="cuda"), return_lse=True)
+    assert out.shape == (0, 8, 128) and lse.shape == (0, 8)
+    got = yr.token_logprobs(torch.empty(0, 50, device="cuda"), torch.empty(0, dtype=torch.int64, device="cuda"), top_k=3)
+    assert got.logprob.shape == (0,) and got.top_token.shape == (0, 3)
+    q = rnd(gen(51), 2, 8, 128)
+    with pytest.raises(N.YpkError, match="out overlaps q"):
+        b.cache.decode(q, out=q)
+    both = torch.zeros(3, 8, 128, dtype=BF16, device="cuda")
+    with pytest.raises(N.YpkError, match="q_out overlaps q"):
+        b.cache.append(rnd(gen(52), 2, 2, 128), rnd(gen(52), 2, 2, 128), q=both[:2], q_out=both[1:])
+    q.requires_grad_()
+    with pytest.raises(ValueError, match="requires a gradient"):
+        b.cache.decode(q)
+    with torch.no_grad():
+        b.cache.decode(q)
 
 
 def prompt_rows(shape, ow, ids):

@@ -151,6 +151,10 @@ def test_c_abi_refuses_before_it_enqueues(native_lib):
     append(c_cache(), N.ERR_INVALID, "row stride 64", rot_dim=128, **dict(table, table_stride=64))
     append(c_cache(), N.ERR_INVALID, "not 16-byte aligned", k=0x10002)
     append(c_cache(), N.ERR_INVALID, "16-byte boundaries", k_stride_token=260)
+    heads = dict(q=0x10000, num_q_heads=8, q_stride_token=1024, q_stride_group=512, q_stride_head=128,
+                 q_out_stride_token=1024, q_out_stride_group=512, q_out_stride_head=128)
+    append(c_cache(), N.ERR_INVALID, "q_out overlaps q", q_out=0x10010, **heads)
+    append(c_cache(), N.ERR_INVALID, "q_out overlaps q", q_out=0x10000, **dict(heads, q_out_stride_token=2048))
     a = N.PagedAppendArgs.from_buffer_copy(args)
     a.num_tokens = 0
     assert lib.ypk_paged_append(C.byref(c_cache()), C.byref(a), None) == N.YPK_OK     # nothing to do
@@ -163,6 +167,8 @@ def test_c_abi_refuses_before_it_enqueues(native_lib):
         assert lib.ypk_paged_decode(C.byref(c), C.byref(a), None) == code
         assert text in lib.ypk_last_error(None).decode(), lib.ypk_last_error(None)
 
+    decode(c_cache(), N.ERR_INVALID, "out overlaps q")
+    decode(c_cache(), N.ERR_INVALID, "out overlaps q", out=0x10000 + 2 * 2 * 1024 - 16)
     decode(c_cache(), N.ERR_INVALID, "3 rows", rows=3)
     decode(c_cache(), N.ERR_INVALID, "7 query heads", num_q_heads=7)
     decode(c_cache(), N.ERR_INVALID, "window -1", window=-1)

@@ -281,7 +281,7 @@ int launch_shape(AppendArgs &a, cudaStream_t st) {
   const auto over = [&](int64_t n, int64_t d) { return (n + d * a.rows_at_once - 1) / (d * a.rows_at_once); };
   const int64_t waves = over(units, int64_t(kResident) * kMaxTurns);
   a.rows_per_cta = std::min(int(over(units, kResident * waves)) * a.rows_at_once, kMaxRows);
-  const dim3 grid((a.tokens + a.rows_per_cta - 1) / a.rows_per_cta, parts(a.heads_per_cta));
+  const dim3 grid(unsigned((int64_t(a.tokens) + a.rows_per_cta - 1) / a.rows_per_cta), parts(a.heads_per_cta));
   if (grid.y > 65535) return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d heads", heads);
   if (a.rows_at_once > 1) paged_append_kernel<T, WIDE_TABLE, D, true><<<grid, kAppendThreads, 0, st>>>(a);
   else paged_append_kernel<T, WIDE_TABLE, D, false><<<grid, kAppendThreads, 0, st>>>(a);
@@ -336,6 +336,15 @@ extern "C" int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_ap
       (p->q && !strides_ok({p->q_stride_token, p->q_stride_group, p->q_stride_head, p->q_out_stride_token,
                             p->q_out_stride_group, p->q_out_stride_head})))
     return op_fail(YPK_ERR_INVALID, "paged_append: rows must start on 16-byte boundaries");
+  const int group = p->q ? p->num_q_heads / cache->num_kv_heads : 1;
+  if (p->q) {
+    // in place or apart: a row is read by the threads that write it, and ahead of that by nobody
+    const HeadRows q = {p->q, p->q_stride_token, p->q_stride_group, p->q_stride_head};
+    const HeadRows out = {p->q_out, p->q_out_stride_token, p->q_out_stride_group, p->q_out_stride_head};
+    const bool same = q.at == out.at && q.token == out.token && q.group == out.group && q.head == out.head;
+    if (!same && heads_touch(q, out, p->num_tokens, cache->num_kv_heads, group, cache->head_dim))
+      return op_fail(YPK_ERR_INVALID, "paged_append: q_out overlaps q without being q");
+  }
   AppendArgs a;
   a.c = paged_view(cache);
   a.q = static_cast<const char *>(p->q);
@@ -353,7 +362,7 @@ extern "C" int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_ap
   a.table_stride = p->table_stride;
   a.tokens = p->num_tokens;
   a.q_heads = p->q ? p->num_q_heads : 0;
-  a.group = p->q ? p->num_q_heads / cache->num_kv_heads : 1;
+  a.group = group;
   a.rot = p->cos ? p->rot_dim : 0;
   a.max_pos = p->max_positions;
   a.eps = p->eps;
