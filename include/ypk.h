@@ -400,7 +400,8 @@ int ypk_argmax_noalloc(const void *logits_bf16, int32_t batch, int32_t vocab, in
  * same paged K/V cache and the same request tables.  Every call is enqueued on `stream` and
  * does not wait; all pointers are device pointers on the current device, the stream's own; the
  * calls allocate nothing, keep nothing from one call for the next and may be captured into a
- * graph.  Arguments that the host can check are refused with YPK_ERR_INVALID or
+ * graph.  Their kernels are launched with programmatic stream serialization and wait for what
+ * runs before them on the stream before they touch memory.  Arguments that the host can check are refused with YPK_ERR_INVALID or
  * YPK_ERR_UNSUPPORTED before anything is enqueued.  What stands in device memory (page numbers,
  * lengths) is checked by the kernels: a broken entry never becomes an address, its token is
  * left out, and a bit of *status tells. */
@@ -470,8 +471,9 @@ typedef struct ypk_paged_decode_args {
   const void *q;                /* [rows][group..][head_dim], grouped as in ypk_paged_append */
   void *out;                    /* like q, apart from it                           */
   float *lse;                   /* [rows][num_q_heads] contiguous, or NULL         */
-  void *workspace;              /* ypk_paged_decode_workspace bytes, 16-byte aligned; holds
-                                   nothing between calls, not shared by calls that overlap */
+  void *workspace;              /* ypk_paged_decode_workspace bytes (NULL if none), 16-byte aligned;
+                                   holds nothing between calls, not shared by calls that
+                                   overlap                                         */
   uint64_t workspace_bytes;
   int64_t q_stride_token, q_stride_group, q_stride_head;
   int64_t out_stride_token, out_stride_group, out_stride_head;
@@ -485,7 +487,8 @@ typedef struct ypk_paged_decode_args {
  * out = sum_p softmax_p(scale q.k_p) v_p, lse = ln sum_p exp(scale q.k_p).  A request without
  * positions gives zeros and -infinity. */
 int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_decode_args *args, void *stream);
-/* Workspace of such a call on the current device for any number of rows and any lengths. */
+/* Workspace of such a call on the current device for any number of rows and any lengths; may
+ * be 0. */
 int ypk_paged_decode_workspace(const ypk_paged_cache *cache, int32_t num_q_heads, uint64_t *bytes);
 
 /* Log probabilities of given tokens under softmax(logits[r, 0:vocab]):

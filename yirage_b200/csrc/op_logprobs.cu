@@ -477,6 +477,7 @@ template <int DTYPE, bool TOP, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
   using V = Vec<DTYPE>;
   using Shared = SharedOf<THREADS>;
+  op_wait_for_previous();
   constexpr int kThreads = THREADS, kWarps = THREADS / 32;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -669,26 +670,13 @@ template <int DTYPE, bool TOP, int THREADS>
 int launch_shape(const LogprobArgs &a, int rows, int device, int sms, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};      // devices where clusters of sixteen have been asked for
   auto *kernel = token_logprobs_kernel<DTYPE, TOP, THREADS>;
-  cudaError_t e = cudaSuccess;
   if (!(ready.load(std::memory_order_relaxed) >> device & 1)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: set-up: %s", cudaGetErrorString(e));
     ready.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
   }
   const int c = cluster_size(rows, a.vocab, sms);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(rows) * c);
-  cfg.blockDim = dim3(THREADS);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = c;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: launch: %s", cudaGetErrorString(e));
-  return YPK_OK;
+  return op_launch("token_logprobs", kernel, dim3(unsigned(rows) * c), THREADS, 0, c, st, a);
 }
 
 // With alternatives wanted and more rows than 256-thread CTAs are resident, CTAs of 128 threads:

@@ -6,6 +6,10 @@
 
 namespace ypk {
 
+// First thing in every kernel of op_launch (op_common.h): until the kernel before it on the stream
+// has ended and its writes are there.
+__device__ __forceinline__ void op_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 struct OpBf16 {
   static __device__ __forceinline__ float2 widen(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));

@@ -140,6 +140,7 @@ __device__ __forceinline__ Place find_place(const AppendArgs &a, int row) {
 // CTAs of 128 threads are resident, each thread with 96 bytes in flight and 96 in work.
 template <class T, bool WIDE_TABLE, int D, bool TOGETHER>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+  op_wait_for_previous();
   constexpr int kLanes = D / 16;                       // threads per head
   constexpr int kItems = kAppendThreads / kLanes;      // heads at a time
   const int at_once = TOGETHER ? a.rows_at_once : 1;
@@ -283,9 +284,10 @@ int launch_shape(AppendArgs &a, cudaStream_t st) {
   a.rows_per_cta = std::min(int(over(units, kResident * waves)) * a.rows_at_once, kMaxRows);
   const dim3 grid(unsigned((int64_t(a.tokens) + a.rows_per_cta - 1) / a.rows_per_cta), parts(a.heads_per_cta));
   if (grid.y > 65535) return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d heads", heads);
-  if (a.rows_at_once > 1) paged_append_kernel<T, WIDE_TABLE, D, true><<<grid, kAppendThreads, 0, st>>>(a);
-  else paged_append_kernel<T, WIDE_TABLE, D, false><<<grid, kAppendThreads, 0, st>>>(a);
-  return op_launched("paged_append");
+  return op_launch("paged_append",
+                   a.rows_at_once > 1 ? paged_append_kernel<T, WIDE_TABLE, D, true>
+                                      : paged_append_kernel<T, WIDE_TABLE, D, false>,
+                   grid, kAppendThreads, 0, 0, st, a);
 }
 
 template <class T, bool WIDE_TABLE>

@@ -156,8 +156,9 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   __shared__ Segment s_start;
   __shared__ float2 s_cta[8 * NT];
 
+  op_wait_for_previous();
   // the joining launch may begin to set itself up; it waits for this grid before it reads
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int heads = a.heads_per_pass;
   char *ring = smem;
@@ -587,7 +588,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   constexpr float kShift = std::is_same<T, OpF16>::value ? 7.f : 0.f;
   __shared__ float2 s_ml[32];
   __shared__ float4 s_o[256];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  op_wait_for_previous();
   const int4 desc = a.desc[blockIdx.x];
   const int parts = desc.z, heads = a.heads_per_pass, h = blockIdx.y;
   const int kv = desc.y / a.head_blocks, h0 = (desc.y % a.head_blocks) * heads;
@@ -677,62 +678,6 @@ uint64_t workspace_bytes(int workers, int heads, int head_dim) {
   return uint64_t(workers) * (16 + 2 * uint64_t(heads) * (8 + 4 * uint64_t(head_dim)));
 }
 
-constexpr int kMaxShared = 232448 - 1024;   // opt-in limit of a block, less the static part
-
-template <class T, int NW, int D, int NT, int S, bool CLUSTER>
-int launch_shape(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
-  using Shape = DecodeShape<NW, D, NT, S>;
-  static std::atomic<uint64_t> ready{0};      // devices whose limit has been raised
-  auto *kernel = paged_decode_kernel<T, NW, D, NT, S, CLUSTER>;
-  cudaError_t e = cudaSuccess;
-  if (!(ready.load(std::memory_order_relaxed) >> dev.device & 1)) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
-    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: shared memory: %s", cudaGetErrorString(e));
-    ready.fetch_or(uint64_t(1) << dev.device, std::memory_order_relaxed);
-  }
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  cfg.gridDim = dim3(dev.sms);
-  cfg.blockDim = dim3(NW * 32);
-  cfg.dynamicSmemBytes = Shape::bytes(a.heads_per_pass, CLUSTER ? 0 : a.rows);
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 0;
-  if (CLUSTER) {
-    cfg.gridDim = dim3(unsigned(a.rows) * a.c.kv_heads * a.head_blocks * a.ctas);
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = a.ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.numAttrs = 1;
-  }
-  e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e == cudaSuccess && !CLUSTER) {
-    // few segments: many threads on each (32 dimensions a block)
-    const int segments = a.rows * a.c.kv_heads * a.head_blocks;
-    const bool fine = a.by_segment && segments * a.heads_per_pass * (D / 32) <= 4 * dev.sms;
-    cfg.gridDim = dim3(a.by_segment ? segments : dev.sms, a.heads_per_pass, fine ? D / 32 : 1);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a);
-  }
-  if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: launch: %s", cudaGetErrorString(e));
-  return YPK_OK;
-}
-
-// Ring depth: three blocks per warp; two where the merge area of sixteen heads or the tables of
-// thousands of requests need the room.
-template <class T, int NW, int D, int NT>
-int launch_ring(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
-  constexpr int kDeep = NT == 2 && D == 128 ? 2 : 3;
-  if (a.ctas) return launch_shape<T, NW, D, NT, kDeep, true>(a, dev, st);
-  if (kDeep == 3 && DecodeShape<NW, D, NT, 3>::bytes(a.heads_per_pass, a.rows) <= kMaxShared)
-    return launch_shape<T, NW, D, NT, kDeep, false>(a, dev, st);
-  return launch_shape<T, NW, D, NT, 2, false>(a, dev, st);
-}
-
 // CTAs per (request, pass) when each gets a cluster of its own, 0: equal ranges.  A cluster is
 // one launch and joins inside it, but a long request among short ones is its cluster's alone.
 // How long it can be is known on the host only as far as the page list goes: clusters are used
@@ -745,6 +690,40 @@ int cluster_ctas(const ypk_paged_cache *c, int rows, int passes, int window, int
   int ctas = 1;
   while (ctas < kMaxCluster && segments * ctas * 2 <= sms && units > 8 * ctas) ctas *= 2;
   return units <= int64_t(kClusterUnits) * ctas && segments * ctas < 0x7fffffff ? ctas : 0;
+}
+
+constexpr int kMaxShared = 232448 - 1024;   // opt-in limit of a block, less the static part
+
+template <class T, int NW, int D, int NT, int S, bool CLUSTER>
+int launch_shape(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
+  using Shape = DecodeShape<NW, D, NT, S>;
+  static std::atomic<uint64_t> ready{0};      // devices whose limit has been raised
+  auto *kernel = paged_decode_kernel<T, NW, D, NT, S, CLUSTER>;
+  if (!(ready.load(std::memory_order_relaxed) >> dev.device & 1)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxShared);
+    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: shared memory: %s", cudaGetErrorString(e));
+    ready.fetch_or(uint64_t(1) << dev.device, std::memory_order_relaxed);
+  }
+  const int shared = Shape::bytes(a.heads_per_pass, CLUSTER ? 0 : a.rows);
+  const unsigned segments = unsigned(a.rows) * a.c.kv_heads * a.head_blocks;
+  if (CLUSTER)
+    return op_launch("paged_decode", kernel, dim3(segments * a.ctas), NW * 32, shared, a.ctas, st, a);
+  if (int rc = op_launch("paged_decode", kernel, dim3(dev.sms), NW * 32, shared, 0, st, a)) return rc;
+  // few segments: many threads on each (32 dimensions a block)
+  const bool fine = a.by_segment && segments * a.heads_per_pass * (D / 32) <= unsigned(4 * dev.sms);
+  return op_launch("paged_decode", paged_join_kernel<T, D>,
+                   dim3(a.by_segment ? segments : dev.sms, a.heads_per_pass, fine ? D / 32 : 1), 256, 0, 0, st, a);
+}
+
+// Ring depth: three blocks per warp; two where the merge area of sixteen heads or the tables of
+// thousands of requests need the room.
+template <class T, int NW, int D, int NT>
+int launch_ring(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
+  constexpr int kDeep = NT == 2 && D == 128 ? 2 : 3;
+  if (a.ctas) return launch_shape<T, NW, D, NT, kDeep, true>(a, dev, st);
+  if (kDeep == 3 && DecodeShape<NW, D, NT, 3>::bytes(a.heads_per_pass, a.rows) <= kMaxShared)
+    return launch_shape<T, NW, D, NT, kDeep, false>(a, dev, st);
+  return launch_shape<T, NW, D, NT, 2, false>(a, dev, st);
 }
 
 template <class T>
@@ -772,7 +751,10 @@ extern "C" int ypk_paged_decode_workspace(const ypk_paged_cache *cache, int32_t 
   if (!bytes) return op_fail(YPK_ERR_INVALID, "paged_decode: null size");
   DeviceInfo dev;
   if (int rc = device_info(&dev)) return rc;
-  *bytes = workspace_bytes(dev.sms, pass_heads(cache->head_dim, num_q_heads / cache->num_kv_heads), cache->head_dim);
+  const int group = num_q_heads / cache->num_kv_heads, heads = pass_heads(cache->head_dim, group);
+  const int passes = cache->num_kv_heads * ((group + heads - 1) / heads);
+  // (fewer rows and a window only make clusters likelier)
+  *bytes = cluster_ctas(cache, cache->num_requests, passes, 0, dev.sms) ? 0 : workspace_bytes(dev.sms, heads, cache->head_dim);
   return YPK_OK;
 }
 
@@ -810,15 +792,15 @@ extern "C" int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_de
   a.window = p->window;
   a.heads_per_pass = pass_heads(cache->head_dim, a.group);
   a.head_blocks = (a.group + a.heads_per_pass - 1) / a.heads_per_pass;
-  a.ctas = cluster_ctas(cache, p->rows, cache->num_kv_heads * a.head_blocks, p->window, dev.sms);
   a.page_div = fast_divisor(cache->page_size);
   a.by_segment = int64_t(p->rows) * cache->num_kv_heads * a.head_blocks <= dev.sms;
   a.scale_log2 = p->scale * 1.4426950408889634f;
-  const uint64_t need = workspace_bytes(dev.sms, a.heads_per_pass, cache->head_dim);
-  if (!p->workspace || p->workspace_bytes < need)
+  a.ctas = cluster_ctas(cache, p->rows, cache->num_kv_heads * a.head_blocks, p->window, dev.sms);
+  const uint64_t need = a.ctas ? 0 : workspace_bytes(dev.sms, a.heads_per_pass, cache->head_dim);
+  if (need && (!p->workspace || p->workspace_bytes < need))
     return op_fail(YPK_ERR_INVALID, "paged_decode: workspace of %llu bytes, %llu needed",
                    (unsigned long long)(p->workspace ? p->workspace_bytes : 0), (unsigned long long)need);
-  char *w = static_cast<char *>(p->workspace);
+  char *w = static_cast<char *>(p->workspace);      // (not used with clusters)
   a.desc = reinterpret_cast<int4 *>(w);
   a.part_o = reinterpret_cast<float *>(w + 16 * uint64_t(dev.sms));
   a.part_ml = reinterpret_cast<float2 *>(a.part_o + 2 * uint64_t(dev.sms) * a.heads_per_pass * cache->head_dim);

@@ -299,7 +299,8 @@ PyObject *paged_decode(PyObject *, PyObject *const *arg, Py_ssize_t n) {
   if (int rc = ypk_paged_decode_workspace(k.c, int32_t(q.heads), &need)) refuse_abi(rc);
   // Of this call alone, from torch's allocator: calls on several streams and graphs that replay
   // at the same time never share it.
-  const c10::DataPtr work = c10::cuda::CUDACachingAllocator::get()->allocate(need);
+  c10::DataPtr work;
+  if (need) work = c10::cuda::CUDACachingAllocator::get()->allocate(need);
   a.q = qt.const_data_ptr();
   a.out = out.data_ptr();
   a.workspace = work.get();
