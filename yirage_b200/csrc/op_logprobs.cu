@@ -266,11 +266,17 @@ __device__ void rank_keys(SharedOf<THREADS> &sh, const unsigned long long *keys,
 // Lists the slots of this thread that reach the bound.
 template <int THREADS>
 __device__ __forceinline__ void list_slots(SharedOf<THREADS> &sh, int slots, uint32_t bound) {
-  for (int i = 0; i < slots; ++i)
-    if (sh.slot_max[i][threadIdx.x] >= bound >> 16) {
-      const int at = atomicAdd(&sh.listed, 1);
-      if (at < kMaxEntries) sh.entry[at] = uint32_t(i) << 16 | threadIdx.x;
-    }
+  for (int i0 = 0; i0 < slots; i0 += 4) {
+    uint32_t most[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most[i] = sh.slot_max[min(i0 + i, slots - 1)][threadIdx.x];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i0 + i < slots && most[i] >= bound >> 16) {
+        const int at = atomicAdd(&sh.listed, 1);
+        if (at < kMaxEntries) sh.entry[at] = uint32_t(i0 + i) << 16 | threadIdx.x;
+      }
+  }
 }
 
 // Puts the columns of this CTA's slice that are at least `least` in order into the list of `to`
@@ -289,8 +295,9 @@ __device__ __forceinline__ void collect(SharedOf<THREADS> &sh, SharedOf<THREADS>
     if (at < kCandidates) to.cand[at] = key_of(o, uint32_t(col));
   };
   for (int i = tid; i < listed * each; i += kThreads) {
-    const uint32_t e = sh.entry[i % listed];
-    const int v = (int(e >> 16) * each + i / listed) * kThreads + int(e & 0xffffu);
+    const int k = each == kUnroll ? i / kUnroll : i / each;
+    const uint32_t e = sh.entry[k];
+    const int v = (int(e >> 16) * each + i - k * each) * kThreads + int(e & 0xffffu);
     if (v >= s.vecs) continue;
     const uint4 x = load16(vec0 + int64_t(v) * 16);
     if (order_of(V::top(x)) < least) continue;
@@ -316,6 +323,7 @@ __device__ __forceinline__ void find_bound(SharedOf<THREADS> &sh, int n, int k) 
   if (tid >= n) return;
   const uint32_t mine = sh.group[tid];
   int above = 0;
+#pragma unroll 8
   for (int j = 0; j < n; j += 4) {
     const uint4 g = *reinterpret_cast<const uint4 *>(sh.group + j);
     above += (g.x > mine) + (g.y > mine) + (g.z > mine) + (g.w > mine);
