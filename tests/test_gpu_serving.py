@@ -777,6 +777,41 @@ def test_two_streams_and_two_graphs_at_once():
     assert same(0, o1) and same(1, o2) and same(2, l1) and same(3, l2)
 
 
+def test_calls_wait_for_what_runs_before_them():
+    """Inputs written just before the call by a long kernel, a copy or a fill on the same stream, or on
+    another one behind an event; outputs read right behind it."""
+    b = Batch([700, 90], [1, 1], page=64, seed=60)
+    g = gen(61)
+    q, n = rnd(g, 2, 8, 128), rnd(g, 2, 2, 128)
+    x, t = rnd(g, 2, 50000), torch.tensor([3, 4], device="cuda")
+    cos, sin = tables(1024, 128, BF16)
+    rotated = b.cache.append(n, n, q=q, cos=cos, sin=sin).clone()
+    want, lp = b.cache.decode(rotated).clone(), yr.token_logprobs(x, t, top_k=4)
+    side, slow = torch.cuda.Stream(), torch.randn(4096, 4096, device="cuda")
+    q2, n2, x2, t2 = torch.empty_like(q), torch.empty_like(n), torch.empty_like(x), torch.empty_like(t)
+    for turn in range(12):
+        for buf in (q2, n2, x2, t2):
+            buf.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side if turn % 2 else torch.cuda.current_stream()):
+            for _ in range(3):
+                slow @ slow
+            x2.copy_(x)
+            t2.copy_(t)
+            n2.copy_(n)
+            q2.copy_(q)
+            if turn % 3 == 0:
+                t2.fill_(3)
+                t2[1:].add_(1)
+        if turn % 2:
+            torch.cuda.current_stream().wait_stream(side)
+        r = b.cache.append(n2, n2, q=q2, cos=cos, sin=sin)
+        o = b.cache.decode(r) + 0
+        p = yr.token_logprobs(x2, t2, top_k=4)
+        for got, right in ((r, rotated), (o, want), (p.logprob * 1, lp.logprob), (p.top_token, lp.top_token)):
+            assert torch.equal(got, right), turn
+
+
 FIRST_CALL = """
 import torch, yirage_b200 as yr
 i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")

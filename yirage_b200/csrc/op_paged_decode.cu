@@ -13,12 +13,22 @@
 // are: the lengths are read on the device, so the same captured launch serves every step.  A
 // (request, head) inside one range is finished there; of one that crosses ranges every CTA
 // leaves (m, sum, O) in the workspace and a second, dependent launch joins them in range order.
-// No atomics: the result does not depend on who comes first.
+// No atomics: the result does not depend on who comes first.  (Joining inside the kernel by
+// whoever comes last measured 2 to 10 us more than the launch: three round trips to L2 with
+// fences between them.)  Where a batch is short, clusters of CTAs take its (request, head)s
+// instead and join through distributed shared memory: one launch, no workspace.
 //
 // Inside a CTA warp w takes the blocks w, w + 8, ...; each warp has its own ring of S blocks in
 // shared memory that it fills with 16-byte cp.async and reads with ldmatrix, so no barrier is
 // needed until a (request, head) ends and the warps' states are merged; the ring runs on
 // across that boundary.
+//
+// Measured, K/V heads of 128, bf16: 64 x 4096 tokens, 32 query / 8 K/V heads 167 us = 6.43 TB/s
+// (98 % of the copy rate); 8 x 4096 30 us = 4.5 TB/s, of which about 9 us are not streaming: launch
+// 1, lengths and range 1.5, page numbers 0.6, first rows 1.5, uneven end 2, merge and join 3;
+// 1 x 513 6.3 us, latency throughout.  What did not help: warps on different K/V heads
+// (64 x 4096 with 64 query heads 184 against 170 us), two CTAs of four warps per SM (8 x 4096 32.6
+// against 30.9), a ring of two blocks (64 x 4096 177 against 169).
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -54,11 +64,15 @@ struct DecodeArgs {
 };
 
 constexpr int kBlock = 16;             // tokens per unit of work
-// Units a CTA should have at least before the work is spread over more CTAs: two per warp.
+// Units a CTA should have at least before the work is spread over more CTAs: two per warp.  (Four:
+// the same within 2 % from 1 x 8192 to 16 x 1000 tokens.)
 constexpr int kMinUnits = 16;
+// Shares shorter than this are cut at the ends of segments if they can be: a second segment in a
+// range costs a merge, 2 to 2.5 us.  16 x 1000 tokens (63 blocks a segment) 17.0 us with the cut
+// moved, 20.3 with equal shares; from 8 x 4096 on equal shares win.
 constexpr int kAlignUnits = 80;
 // Segments of at most this many blocks are not cut: they go whole to the range that holds the
-// larger part of them.
+// larger part of them (64 x 60 tokens, four blocks a segment: 14.6 us, 18.8 with cuts).
 constexpr int kSnapUnits = 16;
 constexpr int kMaxCluster = 8;
 
@@ -681,15 +695,23 @@ uint64_t workspace_bytes(int workers, int heads, int head_dim) {
 // CTAs per (request, pass) when each gets a cluster of its own, 0: equal ranges.  A cluster is
 // one launch and joins inside it, but a long request among short ones is its cluster's alone.
 // How long it can be is known on the host only as far as the page list goes: clusters are used
-// where even the whole list in one request's hands leaves a CTA at most kClusterUnits.
+// where all of them are resident at once (a CTA per SM) and the whole list in one request's hands leaves a CTA at most kClusterUnits.  Measured
+// with equal lengths / with everything in one request, clusters against ranges: 4 x 500 tokens
+// 6.6 against 9.8 / 9.4 against 9.9 us; one step further (a bound of 256) 16 x 100 tokens
+// 5.9 against 7.0 / 20 against 10.
 constexpr int kClusterUnits = 64;
 int cluster_ctas(const ypk_paged_cache *c, int rows, int passes, int window, int sms) {
   int64_t units = (int64_t(c->num_indices) * c->page_size + kBlock - 1) / kBlock;
   if (window > 0) units = std::min(units, int64_t(window) / kBlock + 2);
-  const int64_t segments = int64_t(rows) * passes;
+  // All clusters have to run at once.  One lies in one GPC, and GPCs hold odd numbers of SMs: of 148
+  // SMs, one CTA each, clusters of four reach 132 and of eight 120 on the card measured.  (16 clusters
+  // of eight run in two waves: 1 x 1000 with 16 heads 11.3 us, with four CTAs each 6.4.)
+  const auto resident = [&](int ctas) {
+    return int64_t(rows) * passes * ctas <= (ctas > 4 ? sms * 4 / 5 : ctas > 2 ? sms * 7 / 8 : sms);
+  };
   int ctas = 1;
-  while (ctas < kMaxCluster && segments * ctas * 2 <= sms && units > 8 * ctas) ctas *= 2;
-  return units <= int64_t(kClusterUnits) * ctas && segments * ctas < 0x7fffffff ? ctas : 0;
+  while (ctas < kMaxCluster && resident(ctas * 2) && units > 8 * ctas) ctas *= 2;
+  return units <= int64_t(kClusterUnits) * ctas && resident(ctas) ? ctas : 0;
 }
 
 constexpr int kMaxShared = 232448 - 1024;   // opt-in limit of a block, less the static part
