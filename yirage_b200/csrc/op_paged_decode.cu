@@ -695,16 +695,16 @@ uint64_t workspace_bytes(int workers, int heads, int head_dim) {
 // CTAs per (request, pass) when each gets a cluster of its own, 0: equal ranges.  A cluster is
 // one launch and joins inside it, but a long request among short ones is its cluster's alone.
 // How long it can be is known on the host only as far as the page list goes: clusters are used
-// where all of them are resident at once (a CTA per SM) and the whole list in one request's hands leaves a CTA at most kClusterUnits.  Measured
-// with equal lengths / with everything in one request, clusters against ranges: 4 x 500 tokens
-// 6.6 against 9.8 / 9.4 against 9.9 us; one step further (a bound of 256) 16 x 100 tokens
-// 5.9 against 7.0 / 20 against 10.
+// where all of them are resident at once (a CTA per SM) and the whole list in one request's hands
+// leaves a CTA at most kClusterUnits.  Measured with equal lengths / with everything in one
+// request, clusters against ranges: 4 x 500 tokens 6.6 against 9.8 / 9.4 against 9.9 us; one step
+// further (a bound of 256) 16 x 100 tokens 5.9 against 7.0 / 20 against 10.
 constexpr int kClusterUnits = 64;
 int cluster_ctas(const ypk_paged_cache *c, int rows, int passes, int window, int sms) {
   int64_t units = (int64_t(c->num_indices) * c->page_size + kBlock - 1) / kBlock;
   if (window > 0) units = std::min(units, int64_t(window) / kBlock + 2);
-  // All clusters have to run at once.  One lies in one GPC, and GPCs hold odd numbers of SMs: of 148
-  // SMs, one CTA each, clusters of four reach 132 and of eight 120 on the card measured.  (16 clusters
+  // A cluster lies in one GPC, and GPCs are not multiples of it: of 148 SMs, one CTA each, clusters
+  // of four reach 132 and of eight 120 on the card measured.  (16 clusters
   // of eight run in two waves: 1 x 1000 with 16 heads 11.3 us, with four CTAs each 6.4.)
   const auto resident = [&](int ctas) {
     return int64_t(rows) * passes * ctas <= (ctas > 4 ? sms * 4 / 5 : ctas > 2 ? sms * 7 / 8 : sms);

@@ -117,9 +117,9 @@ class PagedKVCache:
                sm_scale: Optional[float] = None, window: int = 0):
         """Attention of one new token per request: row r of q ([rows, heads, dim] or [rows,
         kv_heads, group, dim], rows <= requests) against all cached positions of request r, or
-        the last `window` of them.  Returns out (shaped like q, not sharing memory with it), or (out, lse [rows, heads]
-        float32) with lse = ln sum_p exp(sm_scale q.k_p); sm_scale defaults to head_dim ** -0.5.
-        A request without positions gives zeros and -inf."""
+        the last `window` of them.  Returns out (shaped like q, not sharing memory with it), or
+        (out, lse [rows, heads] float32) with lse = ln sum_p exp(sm_scale q.k_p); sm_scale
+        defaults to head_dim ** -0.5.  A request without positions gives zeros and -inf."""
         return self._lib.paged_decode(self._at, self._index, q, out, return_lse, sm_scale, window)
 
     def check(self):
