@@ -170,6 +170,23 @@ def test_decode_split_over_long_lengths(hq, heads, lengths):
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)     # no order of arrival in it
 
 
+@pytest.mark.parametrize("page", [1, 2, 7, 16, 48])
+@pytest.mark.parametrize("window", [0, 1500])
+def test_decode_lengths_of_many_short_pages(page, window):
+    """Requests of hundreds of pages beside short ones, from ranges that begin inside them."""
+    run_decode([2500, 1, 650, 0, 1037], page=page, window=window, seed=20 + page)
+    run_decode([700], hq=8, heads=1, dim=256, page=page, window=window, seed=40 + page)
+
+
+def test_decode_many_short_requests_beside_long_ones():
+    """Where the work is cut, the end of every request counts: cuts fall behind the last block of
+    one and inside others."""
+    lengths = [(53 * i) % 420 + (6000 if i in (11, 12, 40) else 0) for i in range(48)]
+    run_decode(lengths, hq=4, heads=4, dim=64, page=16, seed=50)
+    run_decode(lengths[::-1], hq=16, heads=2, dim=128, page=64, seed=51, dtype=F16)
+    run_decode([270] * 37 + [0, 4000], hq=2, heads=1, dim=128, page=16, seed=52)
+
+
 def test_decode_nan_in_a_seen_position_shows():
     """A NaN among the seen K rows makes the heads that read it NaN, and no others."""
     for n, at in ((100, 17), (5000, 4999), (1, 0)):

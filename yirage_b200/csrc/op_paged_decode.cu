@@ -10,7 +10,8 @@
 //
 // Work.  The unit is a block of 16 tokens of one (request, K/V head); all units of the call, in
 // that order, are cut into equal ranges, one per CTA and one CTA per SM, whatever the lengths
-// are: the lengths are read on the device, so the same captured launch serves every step.  A
+// are: the lengths are read on the device, so the same captured launch serves every step.  (The end
+// of a segment counts as work, too: kSegmentUnits.)  A
 // (request, head) inside one range is finished there; of one that crosses ranges every CTA
 // leaves (m, sum, O) in the workspace and a second, dependent launch joins them in range order.
 // No atomics: the result does not depend on who comes first.  (Joining inside the kernel by
@@ -24,7 +25,7 @@
 // across that boundary.
 //
 // Measured, K/V heads of 128, bf16: 64 x 4096 tokens, 32 query / 8 K/V heads 167 us = 6.43 TB/s
-// (98 % of the copy rate); 8 x 4096 30 us = 4.5 TB/s, of which about 9 us are not streaming: launch
+// (98 % of the copy rate); 8 x 4096 29 us = 4.6 TB/s, of which about 8 us are not streaming: launch
 // 1, lengths and range 1.5, page numbers 0.6, first rows 1.5, uneven end 2, merge and join 3;
 // 1 x 513 6.3 us, latency throughout.  What did not help: warps on different K/V heads
 // (64 x 4096 with 64 query heads 184 against 170 us), two CTAs of four warps per SM (8 x 4096 32.6
@@ -74,6 +75,10 @@ constexpr int kAlignUnits = 80;
 // Segments of at most this many blocks are not cut: they go whole to the range that holds the
 // larger part of them (64 x 60 tokens, four blocks a segment: 14.6 us, 18.8 with cuts).
 constexpr int kSnapUnits = 16;
+// What the end of a segment costs a CTA, its merge, in blocks: so much longer a segment counts when
+// the work is cut.  64 requests of 1 to 8192 tokens, where some ranges hold twenty segments and
+// some one: 178 us without, 172 at 8, 170 from 12 to 20, 173 at 28; 8 x 4096 29.6 to 28.9.
+constexpr int kSegmentUnits = 16;
 constexpr int kMaxCluster = 8;
 
 template <class T>
@@ -124,7 +129,8 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
   return (a | b) >> 32 ? a / b : int64_t(uint32_t(a) / uint32_t(b));
 }
 
-// The units of a call cut into equal ranges: worker w's begins at floor(total w / workers).
+// The units of a call cut into equal ranges: worker w's begins at floor(total w / workers).  A
+// segment's units are its blocks and then kSegmentUnits without work.
 struct Ranges {
   int64_t total, each;
   int workers, more;       // total = each workers + more
@@ -204,6 +210,13 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     s.ja = s.ja == 0 || 2 * s.ja <= s.nb ? 0 : s.nb;
     if (s.ja >= s.jb) s.ja = s.jb = 0;
   };
+  // the part of s from unit `at` on, `left` units of the range to go
+  const auto enter_at = [&](Segment &s, int at, int64_t left) {
+    s.ja = min(at, s.nb);
+    s.jb = int(min(int64_t(s.nb), at + left));
+    s.left = max(int64_t(0), at + left - (s.nb + kSegmentUnits));
+    snap(s);
+  };
   Segment begin;
   Ranges all = {};
   int64_t u1 = 0;
@@ -232,8 +245,10 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       if (run.broken && blockIdx.x == 0) paged_flag(a.c, kPagedBadTable);
       s_first[r] = int(run.first);
       s_len[r] = int(run.tokens);
-      mine += int64_t(blocks_of(int(run.tokens))) * passes;
-      requests += run.tokens > 0;
+      if (run.tokens > 0) {
+        mine += int64_t(blocks_of(int(run.tokens)) + kSegmentUnits) * passes;
+        ++requests;
+      }
     }
     int64_t before = mine;            // inclusive scan over the threads
   #pragma unroll
@@ -275,14 +290,12 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       Segment s;
       for (s.r = tid * per;; ++s.r) {
         fill(s);
-        if (off < int64_t(s.nb) * passes) break;
-        off -= int64_t(s.nb) * passes;
+        if (s.nb == 0) continue;
+        if (off < int64_t(s.nb + kSegmentUnits) * passes) break;
+        off -= int64_t(s.nb + kSegmentUnits) * passes;
       }
-      s.pass = int(divide(off, s.nb));
-      s.ja = int(off - int64_t(s.pass) * s.nb);
-      s.jb = int(min(int64_t(s.nb), s.ja + (u1 - u0)));
-      s.left = (u1 - u0) - (s.jb - s.ja);
-      snap(s);
+      s.pass = int(divide(off, s.nb + kSegmentUnits));
+      enter_at(s, int(off - int64_t(s.pass) * (s.nb + kSegmentUnits)), u1 - u0);
       s_start = s;
     }
     if (tid == 0 && !a.by_segment) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -312,10 +325,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       while (s_len[s.r] == 0);
       fill(s);
     }
-    s.ja = 0;
-    s.jb = int(min(int64_t(s.nb), s.left));
-    s.left -= s.jb;
-    snap(s);
+    enter_at(s, 0, s.left);
   };
 
   // ---- filling the ring: this warp's blocks one after the other, across segments
@@ -326,7 +336,20 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   int page = 0, in_page = 0;   // of this lane's row (lane % 16) in the block at the cursor; -1: not seen
   int64_t head_at = 0;         // element offset of the segment's K/V head
   bool more = true;            // the cursor stands on a block
-  const auto enter = [&]() { head_at = fs.pass / a.head_blocks * a.c.stride_head; };
+  // Page numbers come 32 at a time, a lane each, and the next 32 while these are used: the miss of one
+  // load per block shows where pages are short (64 x 4096 in pages of 16: 177 us, so 171).
+  int win = 0, win_next = 0;    // this lane's
+  int at_win = 0, at_next = 0;  // which page of the run lane 0 has
+  int held = 0, last_page = 0;  // blocks that end beyond `held` tokens need other pages; the run's last page
+  const auto pages_from = [&](int q) {
+    return q + lane <= last_page ? __ldg(a.c.indices + fs.first + q + lane) : -1;
+  };
+  const auto enter = [&]() {
+    head_at = fs.pass / a.head_blocks * a.c.stride_head;
+    at_next = -1;
+    held = 0;
+    last_page = fast_div(fs.len - 1, a.page_div);
+  };
   const auto settle = [&]() {  // move the cursor onto a block, fetch its page numbers
     while (fj >= fs.jb) {
       if (fs.left == 0) {
@@ -337,10 +360,29 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       fj = warp;
       enter();
     }
-    const int pos = (fs.b0 + fj) * kBlock + lane % kBlock;
+    const int p0 = (fs.b0 + fj) * kBlock, pos = p0 + lane % kBlock;
     const int q = fast_div(pos, a.page_div);
     in_page = pos < fs.len && pos >= fs.lo ? pos - q * a.c.page_size : -1;
-    page = in_page >= 0 ? __ldg(a.c.indices + fs.first + q) : -1;
+    if constexpr (CLUSTER) {
+      page = in_page >= 0 ? __ldg(a.c.indices + fs.first + q) : -1;
+    } else {
+      if (p0 + kBlock > held) {
+        at_win = fast_div(p0, a.page_div);
+        win = at_win == at_next ? win_next : pages_from(at_win);
+        held = 0x7fffffff;
+        if (last_page - at_win >= 32) {
+          held = (at_win + 32) * a.c.page_size;     // (in the run, so it fits)
+          // the first block of this warp that ends beyond
+          const int p1 = p0 + ((held - p0 - kBlock) / (kBlock * NW) + 1) * (kBlock * NW);
+          at_next = -1;
+          if (p1 < fs.len) {
+            at_next = fast_div(p1, a.page_div);
+            win_next = pages_from(at_next);
+          }
+        }
+      }
+      page = __shfl_sync(~0u, win, (q - at_win) & 31);
+    }
   };
   int fstage = 0;
   const auto issue = [&]() {
