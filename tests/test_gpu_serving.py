@@ -187,6 +187,23 @@ def test_decode_many_short_requests_beside_long_ones():
     run_decode([270] * 37 + [0, 4000], hq=2, heads=1, dim=128, page=16, seed=52)
 
 
+@pytest.mark.parametrize("hq,heads,dim,page,window", [(4, 4, 128, 16, 0), (32, 4, 128, 64, 0), (64, 4, 128, 7, 0),
+                                                      (8, 4, 256, 48, 0), (64, 4, 64, 16, 0), (80, 4, 64, 64, 0),
+                                                      (16, 4, 128, 16, 50), (16, 4, 64, 1, 2000)])
+def test_decode_many_short_requests_warp_by_warp(hq, heads, dim, page, window):
+    """Hundreds of short (request, head)s, a few long ones among them that run through many warps
+    and CTAs: at the start, in the middle, next to one another and at the end."""
+    lengths = [(29 * i) % 131 for i in range(165)]
+    for at, n in ((0, 5000), (80, 2100), (81, 700), (82, 3300), (164, 1500)):
+        lengths[at] = n
+    dtype = F16 if hq == 32 else BF16
+    b, q, out, lse = run_decode(lengths, hq=hq, heads=heads, dim=dim, page=page, window=window, dtype=dtype, seed=70)
+    again = b.cache.decode(q, return_lse=True, window=window)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+    run_decode([1] * 400 + [0] * 7 + [17, 16, 15], hq=hq, heads=heads, dim=dim, page=page, window=window, seed=71)
+    run_decode([512] * 170, hq=hq, heads=heads, dim=dim, page=max(page, 7), window=window, seed=72)
+
+
 def test_decode_nan_in_a_seen_position_shows():
     """A NaN among the seen K rows makes the heads that read it NaN, and no others."""
     for n, at in ((100, 17), (5000, 4999), (1, 0)):

@@ -22,7 +22,8 @@
 // Inside a CTA warp w takes the blocks w, w + 8, ...; each warp has its own ring of S blocks in
 // shared memory that it fills with 16-byte cp.async and reads with ldmatrix, so no barrier is
 // needed until a (request, head) ends and the warps' states are merged; the ring runs on
-// across that boundary.
+// across that boundary.  Where the (request, head)s are many and short, each warp has a range of
+// its own instead (kManyShort) and only what crosses warps is merged, once, at the end.
 //
 // Measured, K/V heads of 128, bf16: 64 x 4096 tokens, 32 query / 8 K/V heads 167 us = 6.43 TB/s
 // (98 % of the copy rate); 8 x 4096 29 us = 4.6 TB/s, of which about 8 us are not streaming: launch
@@ -79,6 +80,18 @@ constexpr int kSnapUnits = 16;
 // the work is cut.  64 requests of 1 to 8192 tokens, where some ranges hold twenty segments and
 // some one: 178 us without, 172 at 8, 170 from 12 to 20, 173 at 28; 8 x 4096 29.6 to 28.9.
 constexpr int kSegmentUnits = 16;
+// Where segments are many and short, each warp has a range of its own and finishes the segments in it
+// by itself, without merges: from kManyShort segments a CTA on if they have up to kShortBlocks
+// blocks on average, from kManyTiny on if up to kTinyBlocks.  Ranges of CTAs against ranges of
+// warps, 8 K/V heads: 256 requests of up to 200 tokens 54.6 / 34.9 us, 148 x 250 39.9 / 33.0, 128 x 512
+// 53.8 / 49.3, 74 x 250 24.5 / 23.6, 64 x 60 16.1 / 12.7; but 64 x 300 27.0 / 28.2, 40 x 250
+// 19.5 / 22.7, 64 x 700 39.9 / 45.3.
+constexpr int kManyShort = 4, kShortBlocks = 32;
+constexpr int kManyTiny = 2, kTinyBlocks = 4;
+// There, what the end of a segment costs a warp, and what is not cut.  (At 16: 256 requests of up to 500
+// tokens 59.7 us against 63.8, but 128 x 512 58.8 against 49.3: merges at every warp's ends.)
+constexpr int kApartEndUnits = 2;
+constexpr int kApartSnapUnits = 32;
 constexpr int kMaxCluster = 8;
 
 template <class T>
@@ -172,8 +185,10 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   constexpr float kShift = std::is_same<T, OpF16>::value ? 7.f : 0.f;
   extern __shared__ __align__(128) char smem[];
   __shared__ int64_t s_warp_total[NW];
-  __shared__ int s_warp_live[NW];
-  __shared__ Segment s_start;
+  __shared__ int64_t s_off[NW];      // where a range begins: units into the request,
+  __shared__ int s_at[NW];           // the request
+  __shared__ int2 s_goes[NW];        // apart: what a warp has of a segment that began before it (Goes, heads)
+  __shared__ int4 s_opens[NW];       // and what it leaves open: request (-1: nothing), pass, blocks to come, heads
   __shared__ float2 s_cta[8 * NT];
 
   op_wait_for_previous();
@@ -202,24 +217,26 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     s.b0 = s.lo / kBlock;
     s.nb = blocks_of(s.len);
   };
+  bool apart = false;                   // each warp has a range of its own (kManyShort)
   // Both ends of a range inside a short segment move to an end of it, the same way for the two
   // ranges that meet there.
   const auto snap = [&](Segment &s) {
-    if (s.nb > kSnapUnits) return;
+    if (s.nb > (apart ? kApartSnapUnits : kSnapUnits)) return;
     s.jb = s.jb == s.nb || 2 * s.jb > s.nb ? s.nb : 0;
     s.ja = s.ja == 0 || 2 * s.ja <= s.nb ? 0 : s.nb;
     if (s.ja >= s.jb) s.ja = s.jb = 0;
   };
+  int end_units = kSegmentUnits;
   // the part of s from unit `at` on, `left` units of the range to go
   const auto enter_at = [&](Segment &s, int at, int64_t left) {
     s.ja = min(at, s.nb);
     s.jb = int(min(int64_t(s.nb), at + left));
-    s.left = max(int64_t(0), at + left - (s.nb + kSegmentUnits));
+    s.left = max(int64_t(0), at + left - (s.nb + end_units));
     snap(s);
   };
   Segment begin;
   Ranges all = {};
-  int64_t u1 = 0;
+  int64_t u0 = 0, u1 = 0;               // this CTA's range, or this warp's
   const int ctas = CLUSTER ? a.ctas : 1, rank = CLUSTER ? int(blockIdx.x) % ctas : 0;
   if (CLUSTER) {
     const int seg = int(blockIdx.x) / ctas;
@@ -236,8 +253,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     begin.left = 0;
   } else {
     const int per = (a.rows + kThreads - 1) / kThreads;
-    int64_t mine = 0;
-    int requests = 0;             // that have positions
+    int64_t mine = 0;             // blocks of a pass, and requests that have positions in the lower 13 bits
     for (int i = 0; i < per; ++i) {
       const int r = tid * per + i;
       if (r >= a.rows) break;
@@ -245,10 +261,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       if (run.broken && blockIdx.x == 0) paged_flag(a.c, kPagedBadTable);
       s_first[r] = int(run.first);
       s_len[r] = int(run.tokens);
-      if (run.tokens > 0) {
-        mine += int64_t(blocks_of(int(run.tokens)) + kSegmentUnits) * passes;
-        ++requests;
-      }
+      mine += (int64_t(blocks_of(int(run.tokens))) << 13) + (run.tokens > 0);
     }
     int64_t before = mine;            // inclusive scan over the threads
   #pragma unroll
@@ -256,48 +269,51 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       const int64_t x = __shfl_up_sync(~0u, before, o);
       if (lane >= o) before += x;
     }
-    requests = __reduce_add_sync(~0u, requests);
-    if (lane == 31) {
-      s_warp_total[warp] = before;
-      s_warp_live[warp] = requests;
-    }
+    if (lane == 31) s_warp_total[warp] = before;
     __syncthreads();
     int64_t total = 0;
-    requests = 0;
     before -= mine;
   #pragma unroll
     for (int w = 0; w < NW; ++w) {
       if (w < warp) before += s_warp_total[w];
       total += s_warp_total[w];
-      requests += s_warp_live[w];
     }
-    all.total = total;
+    const int segments = int(total & 8191) * passes;
+    const int most = segments >= kManyShort * int(gridDim.x)  ? kShortBlocks
+                     : segments >= kManyTiny * int(gridDim.x) ? kTinyBlocks : 0;
+    apart = (total >> 13) * passes <= int64_t(most) * segments;
+    if (apart) end_units = kApartEndUnits;
+    const auto units = [&](int64_t x) { return ((x >> 13) + (x & 8191) * end_units) * passes; };
+    total = units(total);
+    before = units(before);
     // As many workers as have kMinUnits each, or as there are segments; and where a worker's share
     // is short, a whole number per segment, so that equal segments are cut at their ends (a
     // second segment in a range costs about as much as kAlignUnits).
-    const int segments = requests * passes;
     int workers = int(max(int64_t(1), min(max(total / kMinUnits, int64_t(segments)), int64_t(gridDim.x))));
     if (segments > 0 && segments <= workers && total < int64_t(kAlignUnits) * workers)
       workers -= workers % segments;
+    all.total = total;
     all.workers = workers;
     all.each = divide(total, all.workers);
     all.more = int(total - all.each * all.workers);
     const bool works = total > 0 && int(blockIdx.x) < all.workers;
-    const int64_t u0 = all.start(blockIdx.x);
+    u0 = all.start(blockIdx.x);
     u1 = all.start(blockIdx.x + 1);
-    if (works && u0 >= before && u0 < before + mine) {
-      int64_t off = u0 - before;
-      Segment s;
-      for (s.r = tid * per;; ++s.r) {
-        fill(s);
-        if (s.nb == 0) continue;
-        if (off < int64_t(s.nb + kSegmentUnits) * passes) break;
-        off -= int64_t(s.nb + kSegmentUnits) * passes;
+    const int ranges = apart ? NW : 1;
+    if (works && u0 < before + units(mine) && u1 > before)
+      for (int w = 0; w < ranges; ++w) {
+        int64_t off = u0 + (u1 - u0) * w / ranges - before;
+        if (off < 0 || off >= units(mine)) continue;
+        int r = tid * per;
+        for (;; ++r) {
+          if (s_len[r] == 0) continue;
+          const int64_t n = int64_t(blocks_of(s_len[r]) + end_units) * passes;
+          if (off < n) break;
+          off -= n;
+        }
+        s_at[w] = r;
+        s_off[w] = off;
       }
-      s.pass = int(divide(off, s.nb + kSegmentUnits));
-      enter_at(s, int(off - int64_t(s.pass) * (s.nb + kSegmentUnits)), u1 - u0);
-      s_start = s;
-    }
     if (tid == 0 && !a.by_segment) a.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     // requests without positions: nobody's range
     for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
@@ -315,8 +331,23 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     }
     __syncthreads();
     if (!works) return;
-    begin = s_start;
+    if (apart) {
+      const int64_t share = u1 - u0;
+      u1 = u0 + share * (warp + 1) / NW;
+      u0 = u0 + share * warp / NW;
+    }
+    begin.ja = begin.jb = 0;
+    begin.left = 0;
+    if (u0 < u1) {
+      const int w = apart ? warp : 0;
+      begin.r = s_at[w];
+      fill(begin);
+      const int each = begin.nb + end_units;
+      begin.pass = int(divide(s_off[w], each));
+      enter_at(begin, int(s_off[w] - int64_t(begin.pass) * each), u1 - u0);
+    }
   }
+  const int first = apart ? 0 : warp, step = apart ? 1 : NW;   // blocks of a range that this warp takes
 
   const auto next_segment = [&](Segment &s) {   // only while s.left > 0
     if (++s.pass == passes) {
@@ -332,7 +363,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   char *my_ring = ring + warp * (S * 2 * Shape::kTile);
   const uint32_t my_ring32 = static_cast<uint32_t>(__cvta_generic_to_shared(my_ring));
   Segment fs = begin;
-  int fj = fs.ja + warp;
+  int fj = fs.ja + first;
   int page = 0, in_page = 0;   // of this lane's row (lane % 16) in the block at the cursor; -1: not seen
   int64_t head_at = 0;         // element offset of the segment's K/V head
   bool more = true;            // the cursor stands on a block
@@ -357,7 +388,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
         return;
       }
       next_segment(fs);
-      fj = warp;
+      fj = fs.ja + first;
       enter();
     }
     const int p0 = (fs.b0 + fj) * kBlock, pos = p0 + lane % kBlock;
@@ -373,7 +404,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
         if (last_page - at_win >= 32) {
           held = (at_win + 32) * a.c.page_size;     // (in the run, so it fits)
           // the first block of this warp that ends beyond
-          const int p1 = p0 + ((held - p0 - kBlock) / (kBlock * NW) + 1) * (kBlock * NW);
+          const int p1 = p0 + ((held - p0 - kBlock) / (kBlock * step) + 1) * (kBlock * step);
           at_next = -1;
           if (p1 < fs.len) {
             at_next = fast_div(p1, a.page_div);
@@ -404,13 +435,17 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
         copy16(to + Shape::kTile, a.c.v + src, valid);
       }
       fstage = fstage + 1 == S ? 0 : fstage + 1;
-      fj += NW;
+      fj += step;
       settle();
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  enter();
-  settle();
+  if (CLUSTER || u0 < u1) {
+    enter();
+    settle();
+  } else {
+    more = false;
+  }
 #pragma unroll
   for (int s = 0; s < S - 1; ++s) issue();
 
@@ -439,8 +474,33 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     } while (cs.ja >= cs.jb);
     return true;
   };
-  if (!CLUSTER && cs.ja >= cs.jb && !advance()) return;
-  for (;;) {
+  // The state of a warp by itself that goes into a merge: of a segment that began before the warp's
+  // range in its merge area, of one that it opens in its ring, which is empty by then.
+  const auto state_o = [&](int w, bool opened) {
+    return opened ? reinterpret_cast<float *>(ring + w * (S * 2 * Shape::kTile)) : m_o + w * heads * D;
+  };
+  const auto state_ml = [&](int w, bool opened) {
+    return opened ? reinterpret_cast<float2 *>(state_o(w, true) + heads * D) : m_ml + w * heads;
+  };
+  enum Goes { kNone, kOn, kEnds, kEmpty };     // no such segment; it goes on behind the warp; it ends; no range
+  bool some = CLUSTER || cs.ja < cs.jb || advance();
+  if (apart) {
+    if (lane == 0) {
+      s_goes[warp] = make_int2(some ? kNone : kEmpty, 0);
+      s_opens[warp] = make_int4(-1, 0, 0, 0);
+    }
+  } else if (!some) {
+    return;
+  }
+  const auto finish = [&](int r, int kv, int h0, int h, int d, float top, float sum, const float4 &x) {
+    const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+    const uint2 v = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
+    *reinterpret_cast<uint2 *>(a.out + 2 * (r * a.o_token + kv * a.o_group + (h0 + h) * a.o_head + d)) = v;
+    if (a.lse && d == 0)
+      a.lse[int64_t(r) * a.q_heads + kv * a.group + h0 + h] =
+          sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.69314718055994531f;
+  };
+  while (some) {
     load_q(cs);
     const int kv = cs.pass / a.head_blocks, h0 = (cs.pass % a.head_blocks) * heads;
     const int live = min(heads, a.group - h0);        // query heads of this pass
@@ -452,7 +512,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) o[n][d][0] = o[n][d][1] = o[n][d][2] = o[n][d][3] = 0.f;
     }
-    for (int j = cs.ja + warp; j < cs.jb; j += NW) {
+    for (int j = cs.ja + first; j < cs.jb; j += step) {
       asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
       __syncwarp();
       issue();         // into the stage that the previous block has left
@@ -533,17 +593,54 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
         }
       }
     }
-    // ---- merge the warps
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int x = 4; x < 32; x *= 2) l[n][c] += __shfl_xor_sync(~0u, l[n][c], x);
+    if (!CLUSTER && apart && cs.ja == 0 && cs.jb == cs.nb) {
+      // ---- all of the segment: done
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float inv[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const float sum = l[n][c];
+          inv[c] = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+          const int h = n * 8 + (lane % 4) * 2 + c;
+          if (a.lse && lane < 4 && h < live)
+            a.lse[int64_t(cs.r) * a.q_heads + kv * a.group + h0 + h] =
+                sum == 0.f ? -INFINITY : (m[n][c] - kShift + log2f(sum)) * 0.69314718055994531f;
+        }
+        const int h = n * 8 + lane / 4;
+        char *po = a.out + 2 * (cs.r * a.o_token + kv * a.o_group + (h0 + h) * a.o_head) + (lane % 4) * 4;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d) {
+          const uint32_t x0 = transpose8(T::round2(o[n][d][0] * inv[0], o[n][d][1] * inv[1]));
+          const uint32_t x1 = transpose8(T::round2(o[n][d][2] * inv[0], o[n][d][3] * inv[1]));
+          if (h < live) {
+            *reinterpret_cast<uint32_t *>(po + d * 32) = x0;
+            *reinterpret_cast<uint32_t *>(po + d * 32 + 16) = x1;
+          }
+        }
+      }
+      some = advance();
+      continue;
+    }
+    // ---- a part of it: left for the merge
+    const bool opened = !CLUSTER && apart && cs.ja == 0;
+    __syncwarp();
+    float2 *ml = state_ml(warp, opened);
+    float *so = state_o(warp, opened);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int x = 4; x < 32; x *= 2) l[n][c] += __shfl_xor_sync(~0u, l[n][c], x);
         const int h = n * 8 + (lane % 4) * 2 + c;
         if (h < live) {
-          if (lane < 4) m_ml[warp * heads + h] = make_float2(m[n][c], l[n][c]);
-          float *po = m_o + (warp * heads + h) * D + lane / 4;
+          if (lane < 4) ml[h] = make_float2(m[n][c], l[n][c]);
+          float *po = so + h * D + lane / 4;
 #pragma unroll
           for (int d = 0; d < D / 16; ++d) {
             po[d * 16] = o[n][d][c];
@@ -551,6 +648,15 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
           }
         }
       }
+    if (!CLUSTER && apart) {
+      if (lane == 0) {
+        if (opened) s_opens[warp] = make_int4(cs.r, cs.pass, cs.nb - cs.jb, live);
+        else s_goes[warp] = make_int2(cs.jb < cs.nb ? kOn : kEnds, live);
+      }
+      some = advance();
+      continue;
+    }
+    // ---- merge the warps
     __syncthreads();
     const auto warps_joined = [&](int h, int d, float &top, float &sum, float4 &x) {
       top = -INFINITY, sum = 0.f;
@@ -565,14 +671,6 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
         sum += f * ml.y;
         x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
       }
-    };
-    const auto finish = [&](int h, int d, float top, float sum, const float4 &x) {
-      const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
-      const uint2 v = make_uint2(T::round2(x.x * inv, x.y * inv), T::round2(x.z * inv, x.w * inv));
-      *reinterpret_cast<uint2 *>(a.out + 2 * (cs.r * a.o_token + kv * a.o_group + (h0 + h) * a.o_head + d)) = v;
-      if (a.lse && d == 0)
-        a.lse[int64_t(cs.r) * a.q_heads + kv * a.group + h0 + h] =
-            sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.69314718055994531f;
     };
     if (CLUSTER) {
       cg::cluster_group cluster = cg::this_cluster();
@@ -606,7 +704,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
           sum += f * ml[c].y;
           x.x += f * y[c].x, x.y += f * y[c].y, x.z += f * y[c].z, x.w += f * y[c].w;
         }
-        finish(h, d, top, sum, x);
+        finish(cs.r, kv, h0, h, d, top, sum, x);
       }
       cluster.sync();     // nobody leaves while its shared memory is read
       return;
@@ -619,7 +717,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       float4 x;
       warps_joined(h, d, top, sum, x);
       if (whole) {
-        finish(h, d, top, sum, x);
+        finish(cs.r, kv, h0, h, d, top, sum, x);
       } else {
         *reinterpret_cast<float4 *>(a.part_o + (int64_t(slot) * heads + h) * D + d) = x;
         if (d == 0) a.part_ml[int64_t(slot) * heads + h] = make_float2(top, sum);
@@ -630,8 +728,74 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       const int parts = whole ? 0 : all.owner(u1 + (cs.nb - cs.jb) - 1) - int(blockIdx.x) + 1;
       a.desc[a.by_segment ? cs.r * passes + cs.pass : int(blockIdx.x)] = make_int4(cs.r, cs.pass, parts, blockIdx.x);
     }
-    if (!advance()) break;
-    __syncthreads();      // the merge area is free again
+    some = advance();
+    if (some) __syncthreads();      // the merge area is free again
+  }
+  if (!apart) return;
+
+  // ---- segments that warps share: first (c = -1) the one that an earlier CTA began, then what each
+  // warp c opened; in either case with what the next warps have of it
+  __syncthreads();
+  unsigned none = 0, ending = 0, empty = 0, opened = 0;     // a bit per warp
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int goes = s_goes[w].x;
+    none |= unsigned(goes == kNone) << w;
+    ending |= unsigned(goes == kEnds) << w;
+    empty |= unsigned(goes == kEmpty) << w;
+    opened |= unsigned(s_opens[w].x >= 0) << w;
+  }
+  for (int c = -1; c < NW; ++c) {
+    if (c >= 0 && !(opened >> c & 1)) continue;
+    // the warps behind c up to the one that has the segment's end, or the last before one without a part
+    const unsigned behind = ~0u << (c + 1) & ((1u << NW) - 1);
+    const unsigned stop = none & behind, end = ending & behind;
+    const bool ends = end && (!stop || __ffs(end) < __ffs(stop));
+    const unsigned reach = ends ? (end & -end) * 2 - 1 : stop ? (stop & -stop) - 1 : ~0u;
+    const unsigned parts = behind & reach & ~empty;
+    if (c < 0 && !parts) continue;
+    int4 opens = make_int4(0, 0, 0, 0);
+    if (c >= 0) opens = s_opens[c];
+    else opens.w = s_goes[__ffs(parts) - 1].y;
+    const int live = opens.w;
+    const bool whole = c >= 0 && ends;
+    const int kv = opens.y / a.head_blocks, h0 = (opens.y % a.head_blocks) * heads;
+    const int slot = 2 * blockIdx.x + (c >= 0);    // 1: the range that begins the segment
+    for (int i = tid; i < live * (D / 4); i += kThreads) {
+      const int h = i / (D / 4), d = i % (D / 4) * 4;
+      float2 ml[NW];
+      float4 y[NW];
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        ml[w] = make_float2(-INFINITY, 0.f);
+        y[w] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (w == c || (parts >> w & 1)) {
+          ml[w] = state_ml(w, w == c)[h];
+          y[w] = *reinterpret_cast<const float4 *>(state_o(w, w == c) + h * D + d);
+        }
+        top = fmaxf(top, ml[w].x);
+      }
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = ml[w].y == 0.f ? 0.f : exp2_fast(ml[w].x - top);   // (a NaN sum stays one)
+        sum += f * ml[w].y;
+        x.x += f * y[w].x, x.y += f * y[w].y, x.z += f * y[w].z, x.w += f * y[w].w;
+      }
+      if (whole) {
+        finish(opens.x, kv, h0, h, d, top, sum, x);
+      } else {
+        *reinterpret_cast<float4 *>(a.part_o + (int64_t(slot) * heads + h) * D + d) = x;
+        if (d == 0) a.part_ml[int64_t(slot) * heads + h] = make_float2(top, sum);
+      }
+    }
+    if (c >= 0 && tid == 0 && !whole) {
+      // this CTA begins the segment and others go on: how many?
+      const int64_t begins = all.start(blockIdx.x), share = all.start(blockIdx.x + 1) - begins;
+      const int n = all.owner(begins + share * (c + 1) / NW + opens.z - 1) - int(blockIdx.x) + 1;
+      a.desc[blockIdx.x] = make_int4(opens.x, opens.y, n, blockIdx.x);
+    }
   }
 }
 
