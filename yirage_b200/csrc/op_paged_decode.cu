@@ -25,8 +25,8 @@
 // across that boundary.  Where the (request, head)s are many and short, each warp has a range of
 // its own instead (kManyShort) and only what crosses warps is merged, once, at the end.
 //
-// Measured, K/V heads of 128, bf16: 64 x 4096 tokens, 32 query / 8 K/V heads 167 us = 6.43 TB/s
-// (98 % of the copy rate); 8 x 4096 29 us = 4.6 TB/s, of which about 8 us are not streaming: launch
+// Measured, K/V heads of 128, bf16: 64 x 4096 tokens, 32 query / 8 K/V heads 164 us = 6.53 TB/s
+// (99 % of the copy rate); 8 x 4096 29 us = 4.6 TB/s, of which about 8 us are not streaming: launch
 // 1, lengths and range 1.5, page numbers 0.6, first rows 1.5, uneven end 2, merge and join 3;
 // 1 x 513 6.3 us, latency throughout.  What did not help: warps on different K/V heads
 // (64 x 4096 with 64 query heads 184 against 170 us), two CTAs of four warps per SM (8 x 4096 32.6
@@ -58,6 +58,7 @@ struct DecodeArgs {
   FastDivisor page_div;
   float scale_log2;
   // workspace
+  int join_heads;      // a block of the join
   int by_segment;      // the segments are few: desc is indexed by segment, not by worker
   int4 *desc;          // {request, pass, parts, worker}: a segment in several parts, the first that
                        // worker's; parts = 0: nothing to join
@@ -299,10 +300,9 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     const bool works = total > 0 && int(blockIdx.x) < all.workers;
     u0 = all.start(blockIdx.x);
     u1 = all.start(blockIdx.x + 1);
-    const int ranges = apart ? NW : 1;
     if (works && u0 < before + units(mine) && u1 > before)
-      for (int w = 0; w < ranges; ++w) {
-        int64_t off = u0 + (u1 - u0) * w / ranges - before;
+      for (int w = 0; w < (apart ? NW : 1); ++w) {
+        int64_t off = u0 + (u1 - u0) * w / NW - before;
         if (off < 0 || off >= units(mine)) continue;
         int r = tid * per;
         for (;; ++r) {
@@ -799,8 +799,8 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   }
 }
 
-// Joins the parts of one segment (blockIdx.x: see DecodeArgs::by_segment) for query head
-// blockIdx.y of the pass and D / gridDim.z dimensions: parts of workers c (slot 1), c + 1, ...
+// Joins the parts of one segment (blockIdx.x: see DecodeArgs::by_segment) for a.join_heads query
+// heads of the pass and D / gridDim.z dimensions: parts of workers c (slot 1), c + 1, ...
 // (slot 0).  One pass, each group of threads over its own parts, kAhead rows of them in flight.
 template <class T, int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ DecodeArgs a) {
@@ -810,15 +810,18 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   __shared__ float4 s_o[256];
   op_wait_for_previous();
   const int4 desc = a.desc[blockIdx.x];
-  const int parts = desc.z, heads = a.heads_per_pass, h = blockIdx.y;
+  const int parts = desc.z, heads = a.heads_per_pass;
+  if (parts == 0) return;
   const int kv = desc.y / a.head_blocks, h0 = (desc.y % a.head_blocks) * heads;
-  if (parts == 0 || h0 + h >= a.group) return;
   const int lanes = gridDim.z > 1 ? 8 : D / 4;               // threads per row
-  const int groups = 256 / lanes;                            // rows at a time
-  const int g = threadIdx.x / lanes, d = blockIdx.z * 8 + threadIdx.x % lanes;
+  const int groups = 256 / lanes / a.join_heads;             // rows of a head at a time
+  const int row0 = threadIdx.x / lanes / groups * groups;    // the head's first group
+  const int g = threadIdx.x / lanes - row0, d = blockIdx.z * 8 + threadIdx.x % lanes;
+  const int h = blockIdx.y * a.join_heads + row0 / groups;
+  const bool mine = h < heads && h0 + h < a.group;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
   float top = -INFINITY, sum = 0.f;
-  for (int i0 = g; i0 < parts; i0 += groups * kAhead) {
+  for (int i0 = g; mine && i0 < parts; i0 += groups * kAhead) {
     float2 ml[kAhead];
     float4 y[kAhead];
 #pragma unroll
@@ -847,15 +850,15 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     top = next;
   }
   s_o[threadIdx.x] = x;
-  if (threadIdx.x % lanes == 0) s_ml[g] = make_float2(top, sum);
+  if (threadIdx.x % lanes == 0) s_ml[row0 + g] = make_float2(top, sum);
   __syncthreads();
-  if (g != 0) return;
+  if (g != 0 || !mine) return;
   const int used = min(groups, parts);
-  for (int i = 1; i < used; ++i) top = fmaxf(top, s_ml[i].x);
+  for (int i = 1; i < used; ++i) top = fmaxf(top, s_ml[row0 + i].x);
   sum = 0.f;
   x = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < used; ++i) {
-    const float2 ml = s_ml[i];
+    const float2 ml = s_ml[row0 + i];
     const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);
     const float4 y = s_o[i * lanes + threadIdx.x];
     sum += f * ml.y;
@@ -937,10 +940,18 @@ int launch_shape(const DecodeArgs &a, const DeviceInfo &dev, cudaStream_t st) {
   if (CLUSTER)
     return op_launch("paged_decode", kernel, dim3(segments * a.ctas), NW * 32, shared, a.ctas, st, a);
   if (int rc = op_launch("paged_decode", kernel, dim3(dev.sms), NW * 32, shared, 0, st, a)) return rc;
-  // few segments: many threads on each (32 dimensions a block)
-  const bool fine = a.by_segment && segments * a.heads_per_pass * (D / 32) <= unsigned(4 * dev.sms);
+  // Few segments: many threads on each (32 dimensions a block), as long as all blocks find a place
+  // beside the attention kernel's (two per SM; 4 x 1034 tokens 12.0 us, 13.3 with 512 blocks).  Many:
+  // at most one is joined per worker, of two parts as a rule, and blocks for several heads are through
+  // sooner (64 x 4096 166.8 -> 164.3 us; 19 x 6 tokens of 64 heads, nothing to join, 11.5 -> 10.5).
+  const bool fine = a.by_segment && segments * a.heads_per_pass * (D / 32) <= unsigned(2 * dev.sms);
+  DecodeArgs j = a;
+  j.join_heads = 1;
+  if (!a.by_segment)
+    while (j.join_heads < a.heads_per_pass && j.join_heads < 1024 / D) j.join_heads *= 2;
   return op_launch("paged_decode", paged_join_kernel<T, D>,
-                   dim3(a.by_segment ? segments : dev.sms, a.heads_per_pass, fine ? D / 32 : 1), 256, 0, 0, st, a);
+                   dim3(a.by_segment ? segments : dev.sms, (a.heads_per_pass + j.join_heads - 1) / j.join_heads,
+                        fine ? D / 32 : 1), 256, 0, 0, st, j);
 }
 
 // Ring depth: three blocks per warp; two where the merge area of sixteen heads or the tables of
