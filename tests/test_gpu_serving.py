@@ -204,6 +204,40 @@ def test_decode_many_short_requests_warp_by_warp(hq, heads, dim, page, window):
     run_decode([512] * 170, hq=hq, heads=heads, dim=dim, page=max(page, 7), window=window, seed=72)
 
 
+@pytest.mark.parametrize("lengths,heads,hurt,entry", [([100] * 190, 4, 77, 3), ([3000, 60, 3100], 2, 2, 150),
+                                                      ([40] * 300 + [2000], 4, 300, 60)])
+def test_decode_bad_pages_in_either_form(lengths, heads, hurt, entry):
+    """A broken page number, in a batch of many short requests or far into a long one: its request
+    loses those positions, the others keep their bits; an emptied request is zeros."""
+    b = Batch(lengths, heads=heads, page=16, seed=80)
+    q = rnd(gen(81), len(lengths), 4 * heads, 128)
+    good = b.cache.decode(q)
+    b.cache.check()
+    idx, ptr = b.meta["paged_kv_indices_buffer"], b.meta["paged_kv_indptr_buffer"]
+    keep, at = idx.clone(), int(ptr[hurt]) + entry
+    for bad in (-1, b.k.shape[0], 2 ** 31 - 1, -2 ** 31):
+        idx.copy_(keep)
+        idx[at] = bad
+        out = b.cache.decode(q)
+        with pytest.raises(N.YpkError, match="outside the pool"):
+            b.cache.check()
+        others = [r for r in range(len(lengths)) if r != hurt]
+        assert torch.equal(out[others], good[others])
+        pos = torch.arange(lengths[hurt], device="cuda")
+        where = b.where(hurt, pos[(pos < 16 * entry) | (pos >= 16 * (entry + 1))])
+        check_attention(out[hurt], None, q[hurt], b.k[where], b.v[where], 128 ** -0.5, BF16)
+    idx.copy_(keep)
+    b.meta["paged_kv_last_page_len_buffer"][hurt] = 17          # longer than a page
+    out, lse = b.cache.decode(q, return_lse=True)
+    with pytest.raises(N.YpkError, match="out of order"):
+        b.cache.check()
+    assert (out[hurt] == 0).all() and (lse[hurt] == float("-inf")).all()
+    for r in (0, len(lengths) // 2):
+        if r != hurt:
+            where = b.where(r, torch.arange(lengths[r], device="cuda"))
+            check_attention(out[r], lse[r], q[r], b.k[where], b.v[where], 128 ** -0.5, BF16)
+
+
 def test_decode_nan_in_a_seen_position_shows():
     """A NaN among the seen K rows makes the heads that read it NaN, and no others."""
     for n, at in ((100, 17), (5000, 4999), (1, 0)):
