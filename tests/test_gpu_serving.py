@@ -845,6 +845,26 @@ def test_two_streams_and_two_graphs_at_once():
     assert same(0, o1) and same(1, o2) and same(2, l1) and same(3, l2)
 
 
+def test_logprobs_results_stand_by_themselves():
+    """The four results are ordinary contiguous tensors apart from one another, whatever else is done
+    with them."""
+    x, k = rnd(gen(90), 5, 1000), torch.arange(5, device="cuda")
+    keep = [t.clone() for t in yr.token_logprobs(x, k, top_k=3)]
+    for i in range(4):
+        p = yr.token_logprobs(x, k, top_k=3)
+        assert [tuple(t.shape) for t in p] == [(5,), (5,), (5, 3), (5, 3)]
+        assert [t.dtype for t in p] == [F32, F32, F32, torch.int64] and all(t.is_contiguous() for t in p)
+        p[i].zero_()
+        for j in range(4):
+            assert torch.equal(p[j], keep[j] * 0 if i == j else keep[j]), (i, j)
+        copy = p.top_token.to("cpu")
+        del p
+        torch.empty(4096, device="cuda").fill_(7)
+        assert i == 3 or torch.equal(copy, keep[3].cpu())
+    with pytest.raises(N.YpkError, match="top_k"):
+        yr.token_logprobs(x, k, top_k=2 ** 31 - 1)
+
+
 def test_calls_wait_for_what_runs_before_them():
     """Inputs written just before the call by a long kernel, a copy or a fill on the same stream, or on
     another one behind an event; outputs read right behind it."""

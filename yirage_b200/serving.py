@@ -137,6 +137,7 @@ class PagedKVCache:
 
 
 class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns; the four share one allocation."""
     logprob: torch.Tensor                    # [rows] float32
     entropy: torch.Tensor                    # [rows] float32, nats
     top_logprob: Optional[torch.Tensor]      # [rows, top_k] float32, falling (None: top_k = 0)
