@@ -1027,3 +1027,30 @@ def test_prompts_handed_over_to_the_persistent_kernel(max_tokens):
     with pytest.raises(ValueError):
         ypk.token_logprobs(logits, max_tokens + 1)
     ypk.finalize()
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_log_probabilities_of_the_persistent_kernels_own_logits(given):
+    """By default over the vocabulary that the graph samples from: the lm_head of 3000 rows is padded
+    to 4096 with rows of zeros, whose logits are no tokens."""
+    shape = llama.LlamaShape(hidden_size=512, intermediate_size=1024, num_hidden_layers=1, num_attention_heads=8,
+                             num_key_value_heads=2, vocab_size=3000, rms_norm_eps=1e-5)
+    tokens = torch.zeros(2, 64, dtype=torch.int64)
+    tokens[:, :5] = torch.tensor([[5, 100, 2999, 7, 1], [9, 8, 7, 6, 5]])
+    ypk, st = llama.build_decode_kernel(shape, llama.init_weights(shape, "cuda", 5), tokens=tokens.cuda(),
+                                        prompt_lengths=i32([5, 5]), max_num_batched_requests=2,
+                                        max_num_batched_tokens=8, max_num_pages=2, page_size=64)
+    ypk.reset()
+    ypk(max_iterations=4)
+    torch.cuda.synchronize()
+    logits, sampled = st["tensors"]["argmax_in"], st["meta"]["output_tokens"][:2]
+    assert logits.dim(1) == 4096
+    lp = ypk.token_logprobs(logits, 2, top_k=32, **(dict(tokens=sampled) if given else {}))
+    x = ypk.read_tensor(logits)[:2]
+    assert (x[:, 3000:] == 0).all()
+    want = torch.log_softmax(x[:, :3000].to(F64), 1)
+    entropy = -(want.exp() * want).sum(1)
+    assert ((lp.entropy.to(F64) - entropy).abs() <= 2 ** -14 * (1 + entropy)).all()
+    assert ((lp.logprob.to(F64) - want.gather(1, sampled)[:, 0]).abs() <= 2 ** -15 + 2 ** -19).all()
+    assert (lp.top_token < 3000).all() and torch.equal(lp.top_token[:, :1], sampled)
+    ypk.finalize()

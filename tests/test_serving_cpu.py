@@ -271,3 +271,34 @@ def test_cached_prompts_that_cannot_enter_are_refused():
             llama.enter_cached_prompts(Kernel(), state, steps, rows, rows)
     with pytest.raises(ValueError, match="1 layers"):
         llama.enter_cached_prompts(Kernel(), state, [60, 0, 0], rows * 2, rows)
+
+
+def small_kernel(vocab, **kw):
+    ranks = dict(world_size=kw.get("world_size", 1), rank=kw.get("rank", 0))
+    shape = llama.LlamaShape(hidden_size=512, intermediate_size=1024, num_hidden_layers=1, num_attention_heads=8,
+                             num_key_value_heads=2, vocab_size=vocab)
+    return llama.build_decode_kernel(shape, llama.init_weights(shape, "cpu", 0, **ranks),
+                                     tokens=torch.zeros(1, 64, dtype=torch.int64),
+                                     prompt_lengths=torch.tensor([5], dtype=torch.int32), max_num_batched_requests=1,
+                                     max_num_batched_tokens=8, max_num_pages=1, page_size=64, compile=False, **kw)
+
+
+def test_log_probabilities_of_a_graph_are_over_what_it_samples_from():
+    """The lm_head is padded with zero rows to 4096: their logits are no part of the vocabulary."""
+    ypk, state = small_kernel(3000)
+    logits = state["tensors"]["argmax_in"]
+    assert logits.dim(1) == 4096 and ypk._vocabulary_of(logits) == 3000
+    other = state["tensors"]["attn_out"]
+    assert ypk._vocabulary_of(other) == other.dim(1)              # nothing samples from it
+    with pytest.raises(RuntimeError, match="not compiled"):
+        ypk.token_logprobs(logits, 1)
+
+
+@pytest.mark.parametrize("rank", [0, 1])
+def test_log_probabilities_of_a_vocabulary_slice_are_refused(rank):
+    """Sampled tokens are ids of the whole vocabulary, the logits this rank's part of it."""
+    ypk, state = small_kernel(3000, world_size=2, rank=rank)
+    with pytest.raises(ValueError, match="split over the ranks"):
+        ypk.token_logprobs(state["tensors"]["argmax_in"], 1)
+    whole, state = small_kernel(3000, world_size=2, rank=rank, vocab_parallel=False)
+    assert whole._vocabulary_of(state["tensors"]["argmax_in"]) == 3000

@@ -630,22 +630,42 @@ class PersistentKernel:
         self._handle.read_tensor(t.guid, 0, out.data_ptr(), t.nbytes)
         return out
 
+    def _vocabulary_of(self, logits: DTensor) -> int:
+        """Columns of `logits` that are vocabulary, by the arg-max layers that sample from it; all of
+        them where none does.  A rank's slice of a vocabulary that is split is refused."""
+        layers = [(lowering.canonical_name(rt.name), rt.operands, rt.attrs) for rt in self.kn_graph.cygraph.tasks]
+        columns = logits.dim(1)
+        for name, operands, attrs in layers:
+            if name != "argmax_partial" or operands[0] is not logits:
+                continue
+            for other, reads, split in layers:
+                if other == "argmax_reduce" and reads[0] is operands[1] and (
+                        split.get("vocab_offset") or (split.get("exchange") and self.world_size > 1)):
+                    raise ValueError("logits are this rank's slice of a vocabulary that is split over the ranks: "
+                                     "its log probabilities are not those of the sampled tokens")
+            if (attrs.get("valid_cols") or 0) > 0:
+                columns = min(columns, attrs["valid_cols"])
+        return columns
+
     def token_logprobs(self, logits: DTensor, rows: int, tokens: Optional[torch.Tensor] = None,
                        top_k: int = 0, valid_cols: Optional[int] = None):
         """serving.token_logprobs over the first `rows` rows of a logits tensor of the graph as
         the last launch left it, read in place: the log probabilities of what that iteration
         sampled (`tokens`, by default the first `rows` output tokens), its entropy and
-        alternatives."""
+        alternatives.  `valid_cols` is by default what the graph samples from
+        (argmax_partial_layer); logits that are one rank's slice of a split vocabulary are
+        refused."""
         from . import serving
-        if not self._is_compiled or self._dry:
-            raise RuntimeError("PersistentKernel is not compiled for a device")
         if logits.num_dims != 2 or logits.dtype.code not in (N.F16, N.BF16, N.F32):
             raise ValueError("logits must be a [tokens, columns] tensor of bf16, fp16 or fp32")
         if not 0 <= rows <= logits.dim(0):
             raise ValueError(f"{rows} rows of a tensor of {logits.dim(0)}")
-        vocab = logits.dim(1) if valid_cols is None else int(valid_cols)
+        sampled = self._vocabulary_of(logits)
+        vocab = sampled if valid_cols is None else int(valid_cols)
         if not 1 <= vocab <= logits.dim(1):
             raise ValueError(f"valid_cols {vocab} of {logits.dim(1)} columns")
+        if not self._is_compiled or self._dry:
+            raise RuntimeError("PersistentKernel is not compiled for a device")
         if tokens is None:
             tokens = self.meta_tensors["output_tokens"][:rows]
         ptr, _ = self._handle.tensor_ptr(logits.guid)
