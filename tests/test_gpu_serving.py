@@ -1054,3 +1054,75 @@ def test_log_probabilities_of_the_persistent_kernels_own_logits(given):
     assert ((lp.logprob.to(F64) - want.gather(1, sampled)[:, 0]).abs() <= 2 ** -15 + 2 ** -19).all()
     assert (lp.top_token < 3000).all() and torch.equal(lp.top_token[:, :1], sampled)
     ypk.finalize()
+
+
+def check_far_logprobs(x, t, top_k=3):
+    """As check_logprobs, for logits far from zero.  With r = fl(m log2 e) the weights are 2^y,
+    y = fma(x, log2 e, -r): of the largest logit m it is not 0 but some e, |e| <= E = 1.45 u |m|, which the
+    result takes out again.  What is left of it is what numbers of that size are rounded by: log2 s, e
+    and their difference, and a factor of y's own rounding in every weight, 8 u E in all; and in
+    u / s, sums 2^-16 off each, 2^-15 E.  Beyond 2^30 a weight is 0 or 1 and only log2 of a count is rounded."""
+    x64 = x.to(F64)
+    want = torch.log_softmax(x64, 1)
+    p = want.exp()
+    entropy = -torch.where(p > 0, p * want, 0.0).sum(1)
+    top = x64.max(1).values.abs()
+    counted = top > 2.0 ** 30
+    E = torch.where(counted, 0.0, 1.45 * 2 ** -24 * top)
+    base = torch.where(counted, 2.0 ** -20, 2.0 ** -15)
+    got = yr.token_logprobs(x, t, top_k=top_k)
+    at = torch.topk(order_keys(x) * (1 << 20) - torch.arange(x.shape[1], device="cuda"), top_k, 1).indices
+    assert torch.equal(got.top_token, at)
+    for lp, w in ((got.logprob[:, None], want.gather(1, t[:, None])), (got.top_logprob, want.gather(1, at))):
+        lp = lp.to(F64)
+        w = torch.where(torch.isinf(w.to(F32)), float("-inf"), w)            # more than fp32 holds
+        seen = w > float("-inf")
+        assert torch.equal(lp > float("-inf"), seen)
+        bound = base[:, None] * (1 + torch.where(counted[:, None] & seen, w.abs().clamp(max=20.0), 0.0)) \
+            + (8 * 2 ** -24 * E)[:, None] + 2 ** -22 * w.abs()
+        off = (lp - w).abs()
+        assert (off <= bound)[seen].all(), f"log probability off by {off[seen].max().item():.3g}"
+    off = (got.entropy.to(F64) - entropy).abs()
+    bound = torch.where(counted, 2 ** -20 * (1 + entropy), 2 ** -14 * (1 + entropy) + 2 ** -15 * E)
+    assert (off <= bound).all(), f"entropy off by {off.max().item():.3g}"
+
+
+FAR = (100.0, 1000.0, 6e4, 1e6, 5e8, 2.0 ** 30, 1.2e9, 1e10, 1e30)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,vocab", [(3, 9003), (150, 1003), (2, 5)])
+def test_logprobs_far_values_in_the_columns_at_the_ends(dtype, rows, vocab):
+    """Rows that start off a 16-byte boundary, and a vocabulary that ends inside a vector: single columns at
+    both ends.  The largest logit is the first, the last or one in the middle, alone or twice."""
+    g = gen(41)
+    for first in (0, 1, 3, 7):
+        for base in FAR:
+            for sign in (1, -1):
+                if base > torch.finfo(dtype).max:
+                    continue
+                store = torch.full((rows, vocab + 8), float("nan"), dtype=dtype, device="cuda")
+                x = store[:, first:first + vocab]
+                for tops in ((0,), (vocab - 1,), (vocab // 2,), (0, vocab - 1), (0, vocab // 2)):
+                    x.copy_(torch.randn(rows, vocab, generator=g, device="cuda") + sign * base)
+                    step = (x.float().abs().max() * torch.finfo(dtype).eps).item()
+                    x[:, list(tops)] = x.float().max(1, keepdim=True).values.add(max(2.0, 2 * step)).to(dtype)
+                    t = torch.randint(0, vocab, (rows,), generator=g, device="cuda")
+                    t[0] = tops[0]
+                    check_far_logprobs(x, t)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows", [1, 150])
+def test_logprobs_far_values_to_a_rounding(dtype, rows):
+    """Thousands of columns next to the largest logit at every distance from zero, masks below them."""
+    g = gen(42)
+    big = torch.finfo(dtype).max
+    for base in FAR + (2.0 ** 31, 2.3e38, 3.3e38):
+        for sign in (1, -1):
+            if base > big:
+                continue
+            x = (torch.randn(rows, 9000, generator=g, device="cuda") + sign * base).clamp(-big, big).to(dtype)
+            x[:, 7000:] = -big
+            x[:, 8000:] = float("-inf")
+            check_far_logprobs(x, torch.randint(0, 9000, (rows,), generator=g, device="cuda"))

@@ -87,6 +87,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The reference of sums whose largest value is x.  Rounded here and nowhere else: a product that the
+// compiler fused into what is subtracted from it would not be the number that stands in every y.
+__device__ __forceinline__ float reference(float x) { return __fmul_rn(x, kLog2e); }
 __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN on either side stays
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -455,7 +458,7 @@ struct Running {
     if (!(t >= V::kLow)) return t;      // nothing here that counts beside a higher value
     if (t > m) {
       m = t;
-      const float next = t * kLog2e, d = fmaxf(r - next, kFloor);
+      const float next = reference(t), d = fmaxf(r - next, kFloor);
       const float f = exp2_fast(d);
       const f32x2 dd = pair(d, d), ff = pair(f, f);
 #pragma unroll
@@ -558,10 +561,16 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     if (TOP && in_slot > 0) sh.slot_max[slot][tid] = uint16_t(order_of(slot_top) >> 16);
     mine = run.sums();
   }
-  // the single columns at the ends: one per thread
+  // the single columns at the ends: one per thread, against the reference that Running::take has for
+  // such a value, so that the same y of the largest column stands in its weight and in `peak`
   const auto single = [&](int col) {
     const float x = V::one(row + int64_t(col) * V::kBytes);
-    join(mine, x >= V::kLow ? Sums{x * kLog2e, 1.f, 0.f, x} : Sums{-INFINITY, 0.f, 0.f, x});
+    if (!(x >= V::kLow)) {
+      join(mine, Sums{-INFINITY, 0.f, 0.f, x});
+      return;
+    }
+    const float ref = reference(x), y = fmaf(x, kLog2e, -ref), w = exp2_fast(y);
+    join(mine, Sums{ref, w, y * w, x});
   };
   if (tid < s.head) single(s.first + tid);
   if (tid < s.tail) single(s.first + s.head + s.vecs * V::kN + tid);
