@@ -302,3 +302,23 @@ def test_log_probabilities_of_a_vocabulary_slice_are_refused(rank):
         ypk.token_logprobs(state["tensors"]["argmax_in"], 1)
     whole, state = small_kernel(3000, world_size=2, rank=rank, vocab_parallel=False)
     assert whole._vocabulary_of(state["tensors"]["argmax_in"]) == 3000
+
+
+def test_operators_read_with_loads_that_stay_behind_their_wait():
+    """Kernels of op_launch are there while the one before them still writes their inputs.  A load that
+    claims read-only data (.nc, __ldg), or inline assembly that the compiler may move, is not held
+    by the wait in front of it."""
+    csrc = os.path.join(ROOT, "yirage_b200", "csrc")
+    seen = 0
+    for name in sorted(os.listdir(csrc)):
+        if not name.startswith("op_"):
+            continue
+        with open(os.path.join(csrc, name)) as f:
+            code = "\n".join(line.split("//")[0] for line in f)
+        assert "ld.global.nc" not in code and "__ldg(" not in code and "__ldcs(" not in code, name
+        for at in range(len(code)):
+            if code.startswith("ld.global", at):
+                start, end = code.rfind("asm", 0, at), code.index(";", code.index(')', at))
+                assert code.startswith("asm volatile", start) and '"memory"' in code[start:end + 1], (name, code[start:end])
+                seen += 1
+    assert seen >= 3

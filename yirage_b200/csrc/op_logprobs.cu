@@ -97,9 +97,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // a NaN on eithe
 }
 __device__ __forceinline__ uint4 load16(const char *p) {
   uint4 v;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
+}
+// Where `valid`; else v stays.  (By a predicate: the asm in four branches cost two kernels a few bytes
+// of spills.)
+__device__ __forceinline__ void load16_if(uint4 &v, const char *p, bool valid) {
+  asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+               "@q ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+               : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w) : "l"(p), "r"(unsigned(valid)) : "memory");
 }
 
 // One 16-byte vector of logits.
@@ -128,7 +135,7 @@ struct Vec<YPK_F32> {
   static __device__ __forceinline__ float2 two(const uint4 &v, int i) {
     return i ? make_float2(__uint_as_float(v.z), __uint_as_float(v.w)) : make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
   }
-  static __device__ __forceinline__ float one(const char *p) { return __ldg(reinterpret_cast<const float *>(p)); }
+  static __device__ __forceinline__ float one(const char *p) { return *reinterpret_cast<const float *>(p); }
 };
 template <>
 struct Vec<YPK_BF16> {
@@ -159,7 +166,7 @@ struct Vec<YPK_BF16> {
     return OpBf16::widen(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
   }
   static __device__ __forceinline__ float one(const char *p) {
-    return __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16 *>(p)));
+    return __bfloat162float(*reinterpret_cast<const __nv_bfloat16 *>(p));
   }
 };
 template <>
@@ -191,7 +198,7 @@ struct Vec<YPK_F16> {
     return OpF16::widen(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w);
   }
   static __device__ __forceinline__ float one(const char *p) {
-    return __half2float(__ldg(reinterpret_cast<const __half *>(p)));
+    return __half2float(*reinterpret_cast<const __half *>(p));
   }
 };
 
@@ -495,7 +502,6 @@ template <int DTYPE, bool TOP, int THREADS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel(const __grid_constant__ LogprobArgs a) {
   using V = Vec<DTYPE>;
   using Shared = SharedOf<THREADS>;
-  op_wait_for_previous();
   constexpr int kThreads = THREADS, kWarps = THREADS / 32;
   __shared__ Shared sh;
   cg::cluster_group cluster = cg::this_cluster();
@@ -504,18 +510,15 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const char *row = a.logits + r * a.ld * V::kBytes;
   const Slice s = slice_of<DTYPE>(row, a.vocab, rank, ctas);
+  op_wait_for_previous();          // (no memory is touched above)
   const auto meet = [&]() {        // the row's CTAs, or this one's threads
     if (ctas > 1) cluster.sync();
     else __syncthreads();
   };
 
-  // the token's logit is wanted last: ask for it first
   long long token = -1;
   float given = -INFINITY;
-  if (rank == 0 && tid == 0) {
-    token = a.tokens[r];
-    if (token >= 0 && token < a.vocab) given = V::one(row + token * V::kBytes);
-  }
+  if (rank == 0 && tid == 0) token = a.tokens[r];
   if (tid == 0) sh.listed = sh.found = sh.slow = 0;
 
   // ---- the pass: kUnroll vectors per thread at a time, the next ones on their way
@@ -545,7 +548,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     };
     const auto fetch_last = [&]() {
 #pragma unroll
-      for (int j = 0; j < kUnroll; ++j) next[j] = j * kThreads < left ? load16(p + j * (kThreads * 16)) : V::none();
+      for (int j = 0; j < kUnroll; ++j) {
+        next[j] = V::none();
+        load16_if(next[j], p + j * (kThreads * 16), j * kThreads < left);
+      }
     };
     if (whole > 0) fetch_whole();
     else fetch_last();
@@ -561,19 +567,23 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
     if (TOP && in_slot > 0) sh.slot_max[slot][tid] = uint16_t(order_of(slot_top) >> 16);
     mine = run.sums();
   }
-  // the single columns at the ends: one per thread, against the reference that Running::take has for
-  // such a value, so that the same y of the largest column stands in its weight and in `peak`
-  const auto single = [&](int col) {
+  // (wanted at the very end; before the pass its address would have been waited for)
+  if (token >= 0 && token < a.vocab) given = V::one(row + token * V::kBytes);
+  // the single columns at the ends, one per thread of the first and the second warp: against the
+  // reference that Running::take has for such a value, so that the same y of the largest column
+  // stands in its weight and in `peak`
+  const int behind = tid - 32;
+  const int col = tid < s.head ? s.first + tid
+                  : behind >= 0 && behind < s.tail ? s.first + s.head + s.vecs * V::kN + behind : -1;
+  if (col >= 0) {
     const float x = V::one(row + int64_t(col) * V::kBytes);
-    if (!(x >= V::kLow)) {
-      join(mine, Sums{-INFINITY, 0.f, 0.f, x});
-      return;
+    Sums one = {-INFINITY, 0.f, 0.f, x};
+    if (x >= V::kLow) {
+      const float ref = reference(x), y = fmaf(x, kLog2e, -ref), w = exp2_fast(y);
+      one = Sums{ref, w, y * w, x};
     }
-    const float ref = reference(x), y = fmaf(x, kLog2e, -ref), w = exp2_fast(y);
-    join(mine, Sums{ref, w, y * w, x});
-  };
-  if (tid < s.head) single(s.first + tid);
-  if (tid < s.tail) single(s.first + s.head + s.vecs * V::kN + tid);
+    join(mine, one);
+  }
 
   // ---- sums and bounds of the threads, together
   const uint32_t order = order_of(mine.top);

@@ -7,8 +7,19 @@
 namespace ypk {
 
 // First thing in every kernel of op_launch (op_common.h): until the kernel before it on the stream
-// has ended and its writes are there.
+// has ended and its writes are there.  What the kernel before may have written (inputs, page
+// tables, weights: all of it) is read behind this with ordinary loads only: a load that says its
+// data is never written (ld.global.nc, __ldg) may be moved above it, and says something untrue, as
+// this kernel is already there while the one before still writes.
 __device__ __forceinline__ void op_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// 16 bytes that are read once (to leave the caches first).
+__device__ __forceinline__ uint4 op_load_once(const uint4 *p) {
+  uint4 v;
+  asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+  return v;
+}
 
 struct OpBf16 {
   static __device__ __forceinline__ float2 widen(uint32_t v) {

@@ -83,10 +83,10 @@ template <class T, bool WIDE_TABLE>
 __device__ __forceinline__ void load_table(const char *base, int64_t element, f32x2 (&x)[4]) {
   if (WIDE_TABLE) {
     const float4 *p = reinterpret_cast<const float4 *>(base + element * 4);
-    const float4 a = __ldg(p), b = __ldg(p + 1);
+    const float4 a = p[0], b = p[1];
     x[0] = pair(a.x, a.y), x[1] = pair(a.z, a.w), x[2] = pair(b.x, b.y), x[3] = pair(b.z, b.w);
   } else {
-    op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(base + element * 2)), x);
+    op_widen8<T>(*reinterpret_cast<const uint4 *>(base + element * 2), x);
   }
 }
 
@@ -105,22 +105,21 @@ __device__ __forceinline__ Place find_place(const AppendArgs &a, int row) {
   int lo = 0, n = a.c.num_requests;      // the answer is among requests lo .. lo + n
   while (__any_sync(~0u, n > 0)) {
     const int step = (n + LANES - 1) / LANES, at = lo + (lane + 1) * step;
-    const bool before = n > 0 && at <= lo + n && __ldg(a.c.qo + at) <= row;   // requests lo .. at - 1 end before
+    const bool before = n > 0 && at <= lo + n && a.c.qo[at] <= row;   // requests lo .. at - 1 end before
     const int skip = __popc(__ballot_sync(~0u, before) >> shift & ((1u << LANES) - 1)) * step;
     lo += skip;
     n = n > 0 ? min(n - skip, step - 1) : 0;
   }
   Place p = {-1, 0};
   if (lo >= a.c.num_requests) return p;                              // a padding row
-  const PagedRun run = paged_run(__ldg(a.c.indptr + lo), __ldg(a.c.indptr + lo + 1), __ldg(a.c.last + lo),
-                                 a.c.page_size, a.c.num_indices);
-  const int64_t pos = paged_new_position(run, __ldg(a.c.qo + lo + 1), row);
+  const PagedRun run = paged_run(a.c.indptr[lo], a.c.indptr[lo + 1], a.c.last[lo], a.c.page_size, a.c.num_indices);
+  const int64_t pos = paged_new_position(run, a.c.qo[lo + 1], row);
   int bad = 0;
   if (run.broken) bad = kPagedBadTable;
-  else if (__ldg(a.c.qo + lo) > row || pos < 0 || pos >= run.tokens) bad = kPagedBadLength;
+  else if (a.c.qo[lo] > row || pos < 0 || pos >= run.tokens) bad = kPagedBadLength;
   else if (a.cos && pos >= a.max_pos) bad = kPagedBadPosition;
   else {
-    const int q = fast_div(int(pos), a.page_div), page = __ldg(a.c.indices + run.first + q);
+    const int q = fast_div(int(pos), a.page_div), page = a.c.indices[run.first + q];
     p.slot = paged_row(page, a.c.num_pages, int(pos) - q * a.c.page_size, a.c.stride_page, a.c.stride_token);
     p.table = pos * a.table_stride;
     if (p.slot < 0) bad = kPagedBadPage;
@@ -197,8 +196,8 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kern
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (kind[j] >= 0 && t + sub < rows) {
-        n0[j] = __ldcs(reinterpret_cast<const uint4 *>(src[j] + 16 * c0));
-        n1[j] = __ldcs(reinterpret_cast<const uint4 *>(src[j] + 16 * c1));
+        n0[j] = op_load_once(reinterpret_cast<const uint4 *>(src[j] + 16 * c0));
+        n1[j] = op_load_once(reinterpret_cast<const uint4 *>(src[j] + 16 * c1));
       }
       src[j] += src_step[j];
     }
@@ -248,10 +247,10 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kern
           for (int o = kLanes / 2; o; o /= 2) total += __shfl_xor_sync(group_mask, total, o);
           const float f = rsqrtf(total * (1.0f / D) + a.eps);
           f32x2 g[4];
-          op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c0)), g);
+          op_widen8<T>(*reinterpret_cast<const uint4 *>(weight + 16 * c0), g);
 #pragma unroll
           for (int i = 0; i < 4; ++i) u[i] = mul2(mul2(u[i], pair(f, f)), g[i]);
-          op_widen8<T>(__ldg(reinterpret_cast<const uint4 *>(weight + 16 * c1)), g);
+          op_widen8<T>(*reinterpret_cast<const uint4 *>(weight + 16 * c1), g);
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = mul2(mul2(w[i], pair(f, f)), g[i]);
         }

@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
   int at_win = 0, at_next = 0;  // which page of the run lane 0 has
   int held = 0, last_page = 0;  // blocks that end beyond `held` tokens need other pages; the run's last page
   const auto pages_from = [&](int q) {
-    return q + lane <= last_page ? __ldg(a.c.indices + fs.first + q + lane) : -1;
+    return q + lane <= last_page ? a.c.indices[fs.first + q + lane] : -1;
   };
   const auto enter = [&]() {
     head_at = fs.pass / a.head_blocks * a.c.stride_head;
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
     const int q = fast_div(pos, a.page_div);
     in_page = pos < fs.len && pos >= fs.lo ? pos - q * a.c.page_size : -1;
     if constexpr (CLUSTER) {
-      page = in_page >= 0 ? __ldg(a.c.indices + fs.first + q) : -1;
+      page = in_page >= 0 ? a.c.indices[fs.first + q] : -1;
     } else {
       if (p0 + kBlock > held) {
         at_win = fast_div(p0, a.page_div);
@@ -462,8 +462,8 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       const char *qp = a.q + 2 * (s.r * a.q_token + kv * a.q_group + (h0 + h) * a.q_head) + (lane % 4) * 4;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks) {
-        qf[n][ks][0] = h < live ? __ldg(reinterpret_cast<const uint32_t *>(qp + ks * 32)) : 0u;
-        qf[n][ks][1] = h < live ? __ldg(reinterpret_cast<const uint32_t *>(qp + ks * 32 + 16)) : 0u;
+        qf[n][ks][0] = h < live ? *reinterpret_cast<const uint32_t *>(qp + ks * 32) : 0u;
+        qf[n][ks][1] = h < live ? *reinterpret_cast<const uint32_t *>(qp + ks * 32 + 16) : 0u;
       }
     }
   };
