@@ -1126,3 +1126,62 @@ def test_logprobs_far_values_to_a_rounding(dtype, rows):
             x[:, 7000:] = -big
             x[:, 8000:] = float("-inf")
             check_far_logprobs(x, torch.randint(0, 9000, (rows,), generator=g, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("hq,heads,dim,page,lengths", [
+    (8, 2, 128, 64, [200, 30]), (16, 1, 128, 16, [700]), (8, 2, 256, 64, [333, 20]),               # clusters
+    (8, 2, 128, 64, [9000, 40]), (32, 2, 64, 16, [5000, 1, 300]), (16, 2, 256, 3, [4000, 60]),     # ranges
+    (4, 4, 128, 16, [(29 * i) % 131 for i in range(165)] + [3000])])                              # by warps
+def test_decode_infinities_in_v(dtype, hq, heads, dim, page, lengths):
+    """An infinity in V of a seen position is one in its dimension of the output, however small the
+    position's weight is; of both signs, or with a NaN, it is a NaN; other dimensions and heads do not
+    notice, nor does anybody what lies outside the window or behind the end."""
+    g = gen(95)
+    b = Batch(lengths, heads=heads, dim=dim, page=page, dtype=dtype, seed=96)
+    inf, scale = float("inf"), 0.5          # weights down to e^-100 of the largest
+    q = rnd(gen(97), len(lengths), hq, dim, dtype=dtype, scale=3.0)
+    picked = [r for r, n in enumerate(lengths) if n >= 20][:6] + [len(lengths) - 1]
+    clean = b.v.clone()
+    for r in picked:
+        n = lengths[r]
+        at = b.where(r, torch.randperm(n, generator=g, device="cuda")[:8])
+        lo = b.where(r, torch.arange(n, device="cuda"))
+        k = b.k[lo].to(F64)
+        # the position that weighs least in head 0, and the one that weighs most
+        score = torch.einsum("d,ld->l", q[r, 0].to(F64), k[:, 0])
+        ends = b.where(r, torch.stack((score.argmin(), score.argmax())))
+        for a, (place, (dim0, value)) in enumerate(zip([0, 1, 0, 1, 0, 1], [(0, inf), (0, inf), (9, -inf), (17, inf), (17, -inf),
+                                                                        (dim - 1, float("nan"))])):
+            b.v[ends[0][place], ends[1][place], 0, dim0] = value
+        b.v[at[0][0], at[1][0], heads - 1, 5] = -inf
+    out, lse = b.cache.decode(q, return_lse=True, sm_scale=scale)
+    b.cache.check()
+    group = hq // heads
+    for r, n in enumerate(lengths):
+        if not n:
+            continue
+        at = b.where(r, torch.arange(n, device="cuda"))
+        v = b.v[at].to(F64)
+        want = torch.zeros(heads, dim, dtype=F64, device="cuda")
+        up, down, nan = (v == inf).any(0), (v == -inf).any(0), torch.isnan(v).any(0)
+        want[up], want[down], want[nan | (up & down)] = inf, -inf, float("nan")
+        odd = (up | down | nan).repeat_interleave(group, 0)
+        want = want.repeat_interleave(group, 0)
+        got = out[r].to(F64)
+        assert torch.equal(torch.isnan(got), torch.isnan(want)), r
+        assert torch.equal(got[odd & ~torch.isnan(want)], want[odd & ~torch.isnan(want)]), r
+        if r in picked:
+            assert odd.any()
+            check_attention(torch.where(odd, 0.0, got).to(dtype), lse[r], q[r], b.k[at],
+                            torch.where((up | down | nan)[None], 0.0, clean[at].to(F64)).to(dtype), scale, dtype)
+    # the last 5 positions alone, the others holding infinities
+    for r in picked:
+        at = b.where(r, torch.arange(lengths[r] - 5, device="cuda"))
+        b.v[at] = inf
+        at = b.where(r, torch.arange(lengths[r] - 5, lengths[r], device="cuda"))
+        b.v[at] = clean[at]
+    out = b.cache.decode(q, sm_scale=scale, window=5)
+    for r in picked:
+        at = b.where(r, torch.arange(lengths[r] - 5, lengths[r], device="cuda"))
+        check_attention(out[r], None, q[r], b.k[at], b.v[at], scale, dtype)

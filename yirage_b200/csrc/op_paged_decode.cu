@@ -133,6 +133,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Factor of a part's sums when parts are joined.  Never 0 for a part that has weight: an infinity
+// among its sums stays one.  (2^-126 of anything finite is nothing beside the largest weight.)
+__device__ __forceinline__ float part_factor(float part_sum, float part_max, float top) {
+  return part_sum == 0.f ? 0.f : fmaxf(exp2_fast(part_max - top), 0x1p-126f);   // (a NaN sum stays one)
+}
+
 // 16 bytes to shared memory; `valid` false writes zeros and reads nothing.
 __device__ __forceinline__ void copy16(uint32_t dst, const char *src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -173,6 +179,32 @@ struct DecodeShape {
   static int merge_bytes(int heads) { return NW * heads * (8 + D * 4); }
   static int bytes(int heads, int rows) { return kRing + merge_bytes(heads) + NW * S * 4 + rows * 8; }
 };
+
+// Infinities of either sign (a NaN counts as both) that V holds for the positions of blocks j0,
+// j0 + step, ... < j1 of a request: bit d, bit 16 + d: dimension 16 d + lane / 4, and that + 8.
+template <class T, int D>
+__device__ __noinline__ uint2 infinities(const DecodeArgs &a, int first_page, int lo, int len, int j0, int j1,
+                                         int step, int kv) {
+  constexpr uint32_t kExponent = std::is_same<T, OpF16>::value ? 0x7c00u : 0x7f80u;
+  const int lane = threadIdx.x % 32;
+  uint2 found = make_uint2(0u, 0u);
+  for (int j = j0; j < j1; j += step)
+    for (int pos = max(lo, j * kBlock); pos < min(len, (j + 1) * kBlock); ++pos) {
+      const int q = fast_div(pos, a.page_div), page = a.c.indices[first_page + q];
+      const int64_t row = paged_row(page, a.c.num_pages, pos - q * a.c.page_size, a.c.stride_page, a.c.stride_token);
+      if (row < 0) continue;
+      const uint16_t *v = reinterpret_cast<const uint16_t *>(a.c.v) + row + kv * a.c.stride_head + lane / 4;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t x = v[8 * i], size = x & 0x7fffu;
+        if (size < kExponent) continue;
+        const uint32_t bit = 1u << (i / 2 + i % 2 * 16);
+        if (size > kExponent || !(x >> 15)) found.x |= bit;
+        if (size > kExponent || x >> 15) found.y |= bit;
+      }
+    }
+  return found;
+}
 
 // CLUSTER: one cluster of CTAs per (request, pass) instead of equal ranges: the CTAs share its
 // blocks evenly and join through distributed shared memory.  One launch, no workspace.
@@ -599,6 +631,31 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int x = 4; x < 32; x *= 2) l[n][c] += __shfl_xor_sync(~0u, l[n][c], x);
+    // An infinity in V times a weight's two parts may be a NaN: the low part can be negative or 0, and
+    // a weight that is next to nothing has both 0.  Sums that are no numbers though the weights
+    // are: this warp's positions are looked through again, and a dimension that holds an infinity
+    // gets it, one that holds both or a NaN a NaN.
+    float odd[4] = {0.f, 0.f, 0.f, 0.f};       // (four sums: a chain of thirty products showed)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) odd[c] = fmaf(o[n][d][c], 0.f, odd[c]);
+    if (__any_sync(~0u, odd[0] + odd[1] + (odd[2] + odd[3]) != 0.f)) {
+      const uint2 far = infinities<T, D>(a, cs.first, cs.lo, cs.len, cs.b0 + cs.ja + first, cs.b0 + cs.jb, step, kv);
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int bit = d + c / 2 * 16;
+            const bool up = far.x >> bit & 1, down = far.y >> bit & 1;
+            const float sum = l[n][c & 1];
+            if ((up || down) && sum > 0.f) o[n][d][c] = up && down ? NAN : up ? INFINITY : -INFINITY;
+          }
+    }
     if (!CLUSTER && apart && cs.ja == 0 && cs.jb == cs.nb) {
       // ---- all of the segment: done
 #pragma unroll
@@ -666,7 +723,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const float2 ml = m_ml[w * heads + h];
-        const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);   // (a NaN sum stays one)
+        const float f = part_factor(ml.y, ml.x, top);
         const float4 y = *reinterpret_cast<const float4 *>(m_o + (w * heads + h) * D + d);
         sum += f * ml.y;
         x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;
@@ -700,7 +757,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < kMaxCluster; ++c) {
           if (c >= ctas) break;
-          const float f = ml[c].y == 0.f ? 0.f : exp2_fast(ml[c].x - top);
+          const float f = part_factor(ml[c].y, ml[c].x, top);
           sum += f * ml[c].y;
           x.x += f * y[c].x, x.y += f * y[c].y, x.z += f * y[c].z, x.w += f * y[c].w;
         }
@@ -779,7 +836,7 @@ __global__ void __launch_bounds__(NW * 32, 1) paged_decode_kernel(const __grid_c
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        const float f = ml[w].y == 0.f ? 0.f : exp2_fast(ml[w].x - top);   // (a NaN sum stays one)
+        const float f = part_factor(ml[w].y, ml[w].x, top);
         sum += f * ml[w].y;
         x.x += f * y[w].x, x.y += f * y[w].y, x.z += f * y[w].z, x.w += f * y[w].w;
       }
@@ -838,12 +895,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     float next = top;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) next = fmaxf(next, ml[j].x);
-    const float keep = sum == 0.f ? 0.f : exp2_fast(top - next);
+    const float keep = part_factor(sum, top, next);
     sum = sum == 0.f ? 0.f : sum * keep;
     x.x *= keep, x.y *= keep, x.z *= keep, x.w *= keep;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      const float f = ml[j].y == 0.f ? 0.f : exp2_fast(ml[j].x - next);   // (a NaN sum stays one)
+      const float f = part_factor(ml[j].y, ml[j].x, next);
       sum += f * ml[j].y;
       x.x += f * y[j].x, x.y += f * y[j].y, x.z += f * y[j].z, x.w += f * y[j].w;
     }
@@ -859,7 +916,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
   x = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i = 0; i < used; ++i) {
     const float2 ml = s_ml[row0 + i];
-    const float f = ml.y == 0.f ? 0.f : exp2_fast(ml.x - top);
+    const float f = part_factor(ml.y, ml.x, top);
     const float4 y = s_o[i * lanes + threadIdx.x];
     sum += f * ml.y;
     x.x += f * y.x, x.y += f * y.y, x.z += f * y.z, x.w += f * y.w;

@@ -119,7 +119,8 @@ class PagedKVCache:
         kv_heads, group, dim], rows <= requests) against all cached positions of request r, or
         the last `window` of them.  Returns out (shaped like q, not sharing memory with it), or
         (out, lse [rows, heads] float32) with lse = ln sum_p exp(sm_scale q.k_p); sm_scale
-        defaults to head_dim ** -0.5.  A request without positions gives zeros and -inf."""
+        defaults to head_dim ** -0.5.  A request without positions gives zeros and -inf; an
+        infinity in V of a seen position is one in that dimension of out."""
         return self._lib.paged_decode(self._at, self._index, q, out, return_lse, sm_scale, window)
 
     def check(self):
