@@ -1185,3 +1185,24 @@ def test_decode_infinities_in_v(dtype, hq, heads, dim, page, lengths):
     for r in picked:
         at = b.where(r, torch.arange(lengths[r] - 5, lengths[r], device="cuda"))
         check_attention(out[r], None, q[r], b.k[at], b.v[at], scale, dtype)
+
+
+def test_written_tensors_count_their_versions():
+    """What a call writes, autograd takes notice of: a backward pass that saved the old values fails."""
+    b = Batch([30, 20], [1, 1], seed=50)
+    b.k.nan_to_num_(0.5)
+    n, q = rnd(gen(51), 2, 2, 128), rnd(gen(52), 2, 8, 128)
+    out = torch.empty_like(q)
+    w = torch.ones((), device="cuda", requires_grad=True)
+    y = (b.k.float() * w).sum() + (b.k[:1] * w.bfloat16()).float().sum()
+    before = [t._version for t in (b.k, b.v, q, out)]
+    b.cache.append(n, n, q=q, q_out=q)
+    b.cache.decode(q, out=out)
+    assert [t._version - o for t, o in zip((b.k, b.v, q, out), before)] == [1, 1, 1, 1]
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():          # tensors without versions
+        c = Batch([30, 20], [1, 1], seed=50)
+        p = rnd(gen(52), 2, 8, 128)
+        c.cache.decode(c.cache.append(n, n, q=p, q_out=p), out=torch.empty_like(p))
+    assert torch.equal(c.cache.decode(p), out)

@@ -322,3 +322,24 @@ def test_operators_read_with_loads_that_stay_behind_their_wait():
                 assert code.startswith("asm volatile", start) and '"memory"' in code[start:end + 1], (name, code[start:end])
                 seen += 1
     assert seen >= 3
+
+
+def test_forward_mode_tangents_are_refused(native_lib):
+    """The operators have no derivative: a tangent would be lost without a word."""
+    from torch.autograd import forward_ad
+    c = cache()
+    k, q = torch.zeros(2, 2, 128, dtype=torch.bfloat16), torch.zeros(2, 8, 128, dtype=torch.bfloat16)
+    x, t = torch.zeros(4, 100), torch.zeros(4, dtype=torch.int64)
+    with forward_ad.dual_level():
+        dual = lambda a: forward_ad.make_dual(a, torch.ones_like(a))
+        for call in (lambda: c.append(dual(k), k), lambda: c.append(k, dual(k)), lambda: c.append(k, k, q=dual(q)),
+                     lambda: c.append(k, k, q=q, q_out=dual(q)), lambda: c.append(k, k, k_norm=dual(torch.zeros(128).bfloat16())),
+                     lambda: c.decode(dual(q)), lambda: c.decode(q, out=dual(q)), lambda: yr.token_logprobs(dual(x), t),
+                     lambda: yr.PagedKVCache(dual(c.k_cache), c.v_cache, meta()).decode(q)):
+            with pytest.raises(ValueError, match="forward-mode tangent"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU execution path"):
+            c.decode(forward_ad.unpack_dual(dual(q)).primal)
+    grad = yr.PagedKVCache(c.k_cache.requires_grad_(), c.v_cache, meta())
+    with pytest.raises(ValueError, match="k_cache requires a gradient"):
+        grad.decode(q)

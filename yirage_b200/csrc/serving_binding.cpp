@@ -10,6 +10,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -64,7 +65,14 @@ const Tensor &tensor(PyObject *o, const char *name) {
   const Tensor &t = THPVariable_Unpack(o);
   if (t.requires_grad() && at::GradMode::is_enabled())
     refuse(PyExc_ValueError, "%s requires a gradient; the serving operators have none (torch.no_grad or detach)", name);
+  if (t._fw_grad(/*level=*/0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    refuse(PyExc_ValueError, "%s carries a forward-mode tangent; the serving operators have none (detach)", name);
   return t;
+}
+
+// A call has written t: what autograd saved of it for a backward pass is no longer there.
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 const char *type_name(at::ScalarType t) {
@@ -87,6 +95,7 @@ struct Cache {
   c10::Device device;
   at::ScalarType dtype;
   int64_t heads, dim;
+  const Tensor *keys, *values;
 };
 
 int64_t integer(PyObject *o) {
@@ -95,10 +104,12 @@ int64_t integer(PyObject *o) {
   return v;
 }
 
-// `index`: CUDA device of the cache, -1 for the CPU.
-Cache cache_of(PyObject *address, PyObject *index) {
-  Cache k{reinterpret_cast<const ypk_paged_cache *>(integer(address)), c10::Device(c10::kCPU), at::kBFloat16, 0, 0};
-  const int64_t i = integer(index);
+// arg[0]: address of the description; arg[1]: CUDA device of the cache, -1 for the CPU; arg[2], arg[3]:
+// its two tensors.
+Cache cache_of(PyObject *const *arg) {
+  Cache k{reinterpret_cast<const ypk_paged_cache *>(integer(arg[0])), c10::Device(c10::kCPU), at::kBFloat16, 0, 0,
+          &tensor(arg[2], "k_cache"), &tensor(arg[3], "v_cache")};
+  const int64_t i = integer(arg[1]);
   if (i >= 0) k.device = c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(i));
   if (k.c->dtype == YPK_F16) k.dtype = at::kHalf;
   k.heads = k.c->num_kv_heads;
@@ -167,26 +178,26 @@ void kv_rows(const Cache &k, const Tensor &t, const char *name, int64_t *token, 
 
 bool given(PyObject *o) { return o != Py_None; }
 
-// paged_append(cache, device, k, v, q, q_out, cos, sin, q_norm, k_norm, eps) -> q_out or None
+// paged_append(cache, device, k_cache, v_cache, k, v, q, q_out, cos, sin, q_norm, k_norm, eps) -> q_out or None
 PyObject *paged_append(PyObject *, PyObject *const *arg, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 11) refuse(PyExc_TypeError, "paged_append takes 11 arguments");
-  const Cache k = cache_of(arg[0], arg[1]);
-  PyObject *out_obj = arg[5];
+  if (n != 13) refuse(PyExc_TypeError, "paged_append takes 13 arguments");
+  const Cache k = cache_of(arg);
+  PyObject *out_obj = arg[7];
   if (!k.c->qo_indptr) refuse(PyExc_ValueError, "append needs the meta tensor 'qo_indptr_buffer'");
   ypk_paged_append_args a = {};
-  const Tensor &kt = tensor(arg[2], "k"), &vt = tensor(arg[3], "v");
+  const Tensor &kt = tensor(arg[4], "k"), &vt = tensor(arg[5], "v");
   kv_rows(k, kt, "k", &a.k_stride_token, &a.k_stride_head);
   kv_rows(k, vt, "v", &a.v_stride_token, &a.v_stride_head);
   const int64_t tokens = kt.size(0);
   if (vt.size(0) != tokens) refuse(PyExc_ValueError, "k has %lld rows, v %lld", (long long)tokens, (long long)vt.size(0));
   a.num_tokens = int32_t(tokens);
-  const double eps = PyFloat_AsDouble(arg[10]);
+  const double eps = PyFloat_AsDouble(arg[12]);
   if (eps == -1.0 && PyErr_Occurred()) throw python_error();
   a.eps = float(eps);
   Queries q{}, qo{};
-  if (given(arg[4])) {
-    const Tensor &t = tensor(arg[4], "q");
+  if (given(arg[6])) {
+    const Tensor &t = tensor(arg[6], "q");
     q = queries(k, t, "q", false);
     if (q.rows != tokens) refuse(PyExc_ValueError, "q has %lld rows, k %lld", (long long)q.rows, (long long)tokens);
     a.q_stride_token = q.token, a.q_stride_group = q.group, a.q_stride_head = q.head;
@@ -195,12 +206,12 @@ PyObject *paged_append(PyObject *, PyObject *const *arg, Py_ssize_t n) {
       qo = queries(k, tensor(out_obj, "q_out"), "q_out", true);
       if (qo.rows != tokens || qo.heads != q.heads) refuse(PyExc_ValueError, "q_out must have the rows and heads of q");
     }
-  } else if (given(out_obj) || given(arg[8])) {
+  } else if (given(out_obj) || given(arg[10])) {
     refuse(PyExc_ValueError, "q_out and q_norm come with q");
   }
-  if (given(arg[6]) != given(arg[7])) refuse(PyExc_ValueError, "cos and sin come together");
-  if (given(arg[6])) {
-    const Tensor &c = tensor(arg[6], "cos"), &s = tensor(arg[7], "sin");
+  if (given(arg[8]) != given(arg[9])) refuse(PyExc_ValueError, "cos and sin come together");
+  if (given(arg[8])) {
+    const Tensor &c = tensor(arg[8], "cos"), &s = tensor(arg[9], "sin");
     if ((c.scalar_type() != k.dtype && c.scalar_type() != at::kFloat) || s.scalar_type() != c.scalar_type())
       refuse(PyExc_TypeError, "cos and sin must both be of the cache's type or float32");
     if (c.dim() != 2 || c.sizes() != s.sizes() || c.strides() != s.strides() || c.stride(1) != 1 ||
@@ -213,9 +224,9 @@ PyObject *paged_append(PyObject *, PyObject *const *arg, Py_ssize_t n) {
     a.rot_dim = int32_t(c.size(1));
     a.table_stride = c.size(0) > 1 ? c.stride(0) : (c.size(1) + 7) / 8 * 8;
   }
-  for (int i = 8; i < 10; ++i) {
+  for (int i = 10; i < 12; ++i) {
     if (!given(arg[i])) continue;
-    const char *name = i == 8 ? "q_norm" : "k_norm";
+    const char *name = i == 10 ? "q_norm" : "k_norm";
     const Tensor &w = tensor(arg[i], name);
     operand(k, w, name);
     if (w.dim() != 1 || w.size(0) != k.dim || !w.is_contiguous())
@@ -224,7 +235,7 @@ PyObject *paged_append(PyObject *, PyObject *const *arg, Py_ssize_t n) {
   need_cuda(k.device);
   const c10::cuda::CUDAGuard guard(k.device);
   Tensor made;
-  if (given(arg[4])) {
+  if (given(arg[6])) {
     if (given(out_obj)) {
       a.q_out = THPVariable_Unpack(out_obj).data_ptr();
       a.q_out_stride_token = qo.token, a.q_out_stride_group = qo.group, a.q_out_stride_head = qo.head;
@@ -235,55 +246,58 @@ PyObject *paged_append(PyObject *, PyObject *const *arg, Py_ssize_t n) {
       a.q_out_stride_group = q.heads / k.heads * k.dim;
       a.q_out_stride_head = k.dim;
     }
-    a.q = THPVariable_Unpack(arg[4]).const_data_ptr();
+    a.q = THPVariable_Unpack(arg[6]).const_data_ptr();
   }
   a.k = kt.const_data_ptr();
   a.v = vt.const_data_ptr();
-  if (given(arg[6])) {
-    a.cos = THPVariable_Unpack(arg[6]).const_data_ptr();
-    a.sin = THPVariable_Unpack(arg[7]).const_data_ptr();
+  if (given(arg[8])) {
+    a.cos = THPVariable_Unpack(arg[8]).const_data_ptr();
+    a.sin = THPVariable_Unpack(arg[9]).const_data_ptr();
   }
-  if (given(arg[8])) a.q_norm = THPVariable_Unpack(arg[8]).const_data_ptr();
-  if (given(arg[9])) a.k_norm = THPVariable_Unpack(arg[9]).const_data_ptr();
+  if (given(arg[10])) a.q_norm = THPVariable_Unpack(arg[10]).const_data_ptr();
+  if (given(arg[11])) a.k_norm = THPVariable_Unpack(arg[11]).const_data_ptr();
   void *stream = c10::cuda::getCurrentCUDAStream(k.device.index()).stream();
   call_abi([&] { return ypk_paged_append(k.c, &a, stream); });
+  written(*k.keys);
+  written(*k.values);
+  if (given(out_obj)) written(THPVariable_Unpack(out_obj));
   if (made.defined()) return THPVariable_Wrap(std::move(made));
   return Py_NewRef(out_obj);      // None without queries
   END_HANDLE_TH_ERRORS
 }
 
-// paged_decode(cache, device, q, out, return_lse, sm_scale, window) -> out or (out, lse)
+// paged_decode(cache, device, k_cache, v_cache, q, out, return_lse, sm_scale, window) -> out or (out, lse)
 PyObject *paged_decode(PyObject *, PyObject *const *arg, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 7) refuse(PyExc_TypeError, "paged_decode takes 7 arguments");
-  const Cache k = cache_of(arg[0], arg[1]);
-  const Tensor &qt = tensor(arg[2], "q");
+  if (n != 9) refuse(PyExc_TypeError, "paged_decode takes 9 arguments");
+  const Cache k = cache_of(arg);
+  const Tensor &qt = tensor(arg[4], "q");
   const Queries q = queries(k, qt, "q", false);
   if (q.rows > k.c->num_requests)
     refuse(PyExc_ValueError, "q has %lld rows, the tables %d requests", (long long)q.rows, k.c->num_requests);
   Queries o{};
-  if (given(arg[3])) {
-    const Tensor &t = tensor(arg[3], "out");
+  if (given(arg[5])) {
+    const Tensor &t = tensor(arg[5], "out");
     if (t.sizes() != qt.sizes()) refuse(PyExc_ValueError, "out must have the shape of q");
     o = queries(k, t, "out", true);
   }
-  const int lse_wanted = PyObject_IsTrue(arg[4]);
+  const int lse_wanted = PyObject_IsTrue(arg[6]);
   if (lse_wanted < 0) throw python_error();
   ypk_paged_decode_args a = {};
   a.scale = 1.0f / sqrtf(float(k.dim));
-  if (given(arg[5])) {
-    const double s = PyFloat_AsDouble(arg[5]);
+  if (given(arg[7])) {
+    const double s = PyFloat_AsDouble(arg[7]);
     if (s == -1.0 && PyErr_Occurred()) throw python_error();
     a.scale = float(s);
   }
-  const int64_t window = integer(arg[6]);
+  const int64_t window = integer(arg[8]);
   if (window < 0) refuse(PyExc_ValueError, "window %lld is negative", (long long)window);
   a.window = int32_t(std::min<int64_t>(window, 0x7fffffff));
   need_cuda(k.device);
   const c10::cuda::CUDAGuard guard(k.device);
   Tensor out, lse;
-  if (given(arg[3])) {
-    out = THPVariable_Unpack(arg[3]);
+  if (given(arg[5])) {
+    out = THPVariable_Unpack(arg[5]);
     a.out_stride_token = o.token, a.out_stride_group = o.group, a.out_stride_head = o.head;
   } else {
     out = at::detail::empty_cuda(qt.sizes(), k.dtype, k.device, std::nullopt);
@@ -310,7 +324,8 @@ PyObject *paged_decode(PyObject *, PyObject *const *arg, Py_ssize_t n) {
   a.num_q_heads = int32_t(q.heads);
   void *stream = c10::cuda::getCurrentCUDAStream(k.device.index()).stream();
   call_abi([&] { return ypk_paged_decode(k.c, &a, stream); });
-  PyObject *first = given(arg[3]) ? Py_NewRef(arg[3]) : THPVariable_Wrap(std::move(out));
+  if (given(arg[5])) written(out);
+  PyObject *first = given(arg[5]) ? Py_NewRef(arg[5]) : THPVariable_Wrap(std::move(out));
   if (!lse_wanted || !first) return first;
   PyObject *second = THPVariable_Wrap(std::move(lse));
   PyObject *both = second ? PyTuple_Pack(2, first, second) : nullptr;

@@ -111,7 +111,8 @@ class PagedKVCache:
         their positions: 32-bit arithmetic, one rounding.  Any strides that keep rows on
         16-byte boundaries.  Returns the rotated q (`q_out`, which may be q itself, or a new
         tensor); its rows behind qo_indptr[requests] are not written."""
-        return self._lib.paged_append(self._at, self._index, k, v, q, q_out, cos, sin, q_norm, k_norm, eps)
+        return self._lib.paged_append(self._at, self._index, self.k_cache, self.v_cache, k, v, q, q_out, cos, sin,
+                                      q_norm, k_norm, eps)
 
     def decode(self, q: torch.Tensor, *, out: Optional[torch.Tensor] = None, return_lse: bool = False,
                sm_scale: Optional[float] = None, window: int = 0):
@@ -121,7 +122,8 @@ class PagedKVCache:
         (out, lse [rows, heads] float32) with lse = ln sum_p exp(sm_scale q.k_p); sm_scale
         defaults to head_dim ** -0.5.  A request without positions gives zeros and -inf; an
         infinity in V of a seen position is one in that dimension of out."""
-        return self._lib.paged_decode(self._at, self._index, q, out, return_lse, sm_scale, window)
+        return self._lib.paged_decode(self._at, self._index, self.k_cache, self.v_cache, q, out, return_lse, sm_scale,
+                                      window)
 
     def check(self):
         """Wait for the work enqueued so far on the current stream and raise if a call found a
