@@ -343,3 +343,17 @@ def test_forward_mode_tangents_are_refused(native_lib):
     grad = yr.PagedKVCache(c.k_cache.requires_grad_(), c.v_cache, meta())
     with pytest.raises(ValueError, match="k_cache requires a gradient"):
         grad.decode(q)
+
+
+def test_a_cache_that_has_moved_is_refused(native_lib):
+    """Calls go where the cache was when it was described: not after its memory was exchanged."""
+    k, q = torch.zeros(2, 2, 128, dtype=torch.bfloat16), torch.zeros(2, 8, 128, dtype=torch.bfloat16)
+    for move in (lambda c: c.k_cache.resize_(400, 16, 2, 128), lambda c: c.v_cache.set_(c.v_cache.clone()),
+                 lambda c: setattr(c, "k_cache", c.k_cache.clone())):
+        c = cache()
+        with pytest.raises(RuntimeError, match="no CPU execution path"):
+            c.decode(q)
+        move(c)
+        for call in (lambda: c.decode(q), lambda: c.append(k, k)):
+            with pytest.raises(ValueError, match="not where it was"):
+                call()

@@ -109,6 +109,9 @@ int64_t integer(PyObject *o) {
 Cache cache_of(PyObject *const *arg) {
   Cache k{reinterpret_cast<const ypk_paged_cache *>(integer(arg[0])), c10::Device(c10::kCPU), at::kBFloat16, 0, 0,
           &tensor(arg[2], "k_cache"), &tensor(arg[3], "v_cache")};
+  // (data_ptr of a tensor whose storage was resized or exchanged: the description points elsewhere)
+  if (k.keys->const_data_ptr() != k.c->k || k.values->const_data_ptr() != k.c->v)
+    refuse(PyExc_ValueError, "k_cache or v_cache is not where it was when PagedKVCache was made");
   const int64_t i = integer(arg[1]);
   if (i >= 0) k.device = c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(i));
   if (k.c->dtype == YPK_F16) k.dtype = at::kHalf;

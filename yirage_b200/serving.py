@@ -61,7 +61,8 @@ class PagedKVCache:
     call, qo_indptr_buffer [requests + 1] by append().  Request r is (its pages - 1) *
     page_size + last_page_len[r] tokens long, new tokens included; no pages: an empty slot.
     The tables' contents may change between calls (and between replays of a graph); the
-    tensors themselves stay the caller's and are kept alive, unmoved, by this object.
+    tensors themselves stay the caller's, are kept alive by this object and must stay where they
+    are: a cache whose memory was exchanged since (resize_, set_) is refused.
 
     Broken table entries never become addresses: their tokens are left out and a bit is set in
     `status` (int32 [1] on the device), which check() reads."""
