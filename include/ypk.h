@@ -463,7 +463,9 @@ typedef struct ypk_paged_append_args {
  * h = rot_dim / 2, in 32 bits with one rounding at the end.  Rows of k, v and q behind
  * qo_indptr[num_requests] are not read into anything; the rows of q_out there stay as they
  * were, and so do those of dropped tokens.  Two rows of a call must not go to the same place (two
- * requests that share a last page). */
+ * requests that share a last page).  Refused: caches whose rows lie on one another, K on V among
+ * them, and q_out on q (without being q), k, v or the cache; rows that alternate in one buffer
+ * without touching are apart. */
 int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_append_args *args, void *stream);
 
 /* Operands of ypk_paged_decode. */

@@ -1206,3 +1206,30 @@ def test_written_tensors_count_their_versions():
         p = rnd(gen(52), 2, 8, 128)
         c.cache.decode(c.cache.append(n, n, q=p, q_out=p), out=torch.empty_like(p))
     assert torch.equal(c.cache.decode(p), out)
+
+
+def test_queries_and_outputs_side_by_side_in_one_buffer():
+    """Rows of q and of what is written that alternate in memory without touching."""
+    b = Batch([50, 80, 20], [1, 1, 1], heads=2, seed=13)
+    g = gen(14)
+    cos, sin = tables(128, 128, BF16)
+    rows = rnd(g, 3, 2, 4 + 4 + 2, 128)
+    q, out, k, v = rows[:, :, :4], rows[:, :, 4:8], rows[:, :, 8], rows[:, :, 9]
+    before = rows.clone()
+    want = b.cache.append(k, v, q=q.clone(), cos=cos, sin=sin)
+    assert b.cache.append(k, v, q=q, q_out=out, cos=cos, sin=sin).data_ptr() == out.data_ptr()
+    same = lambda: torch.equal(rows[:, :, :4], before[:, :, :4]) and torch.equal(rows[:, :, 8:], before[:, :, 8:])
+    assert torch.equal(out.reshape(3, 8, 128), want) and same()
+    want = b.cache.decode(q.clone())
+    b.cache.decode(q, out=out)
+    assert torch.equal(out, want) and same()
+    both = rnd(g, 3, 2, 8, 128)                      # whole heads alternate
+    want = b.cache.decode(both[:, 0].clone())
+    b.cache.decode(both[:, 0], out=both[:, 1])
+    assert torch.equal(both[:, 1], want)
+    with pytest.raises(N.YpkError, match="q_out overlaps k or v"):
+        b.cache.append(k, v, q=q, q_out=rows[:, :, 5:9], cos=cos, sin=sin)
+    same = yr.PagedKVCache(b.k, b.k, b.meta)         # read as K and V alike, not written as both
+    assert torch.equal(same.decode(q), yr.PagedKVCache(b.k, b.k.clone(), b.meta).decode(q))
+    with pytest.raises(N.YpkError, match="K and V rows"):
+        same.append(k, v)

@@ -357,3 +357,111 @@ def test_a_cache_that_has_moved_is_refused(native_lib):
         for call in (lambda: c.decode(q), lambda: c.append(k, k)):
             with pytest.raises(ValueError, match="not where it was"):
                 call()
+
+
+OVERLAPS = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <set>
+#include "strided_rows.h"
+using namespace ypk;
+static std::set<int64_t> starts(const StridedRows &r, bool &twice) {
+  std::set<int64_t> s;
+  for (int64_t i = 0; i < r.count[0]; ++i) for (int64_t j = 0; j < r.count[1]; ++j) for (int64_t k = 0; k < r.count[2]; ++k)
+    twice |= !s.insert(r.at + i * r.stride[0] + j * r.stride[1] + k * r.stride[2]).second;
+  return s;
+}
+int main() {
+  std::mt19937 g(1);
+  const auto pick = [&](int lo, int hi) { return int64_t(lo + g() % (hi - lo + 1)); };
+  int met = 0, apart = 0, close = 0, loose = 0;
+  for (int turn = 0; turn < 60000; ++turn) {
+    StridedRows a = {pick(0, 60), pick(1, 8), {}, {}}, b = a;
+    for (int k = 0; k < 3; ++k) {
+      a.stride[k] = pick(0, turn % 2 ? 40 : 12);
+      a.count[k] = pick(1, 5);
+      b.stride[k] = pick(0, 3) ? a.stride[k] : pick(0, 40);
+      b.count[k] = pick(0, 3) ? a.count[k] : pick(0, 5);
+    }
+    b.at = pick(0, 120);
+    bool twice = false, unused = false;
+    const auto sa = starts(a, twice), sb = starts(b, unused);
+    for (auto i = sa.begin(); i != sa.end() && std::next(i) != sa.end(); ++i) twice |= *std::next(i) - *i < a.width;
+    bool touch = false;
+    for (int64_t x : sa) { const auto i = sb.lower_bound(x - a.width + 1); touch |= i != sb.end() && *i < x + a.width; }
+    if (rows_distinct(a) == twice || rows_touch(a, b) != touch || rows_touch(b, a) != touch) {
+      std::printf("turn %d: distinct %d, by hand %d; touch %d, by hand %d\n", turn, rows_distinct(a), !twice, rows_touch(a, b), touch);
+      return 1;
+    }
+    (touch ? met : apart)++;
+    (twice ? close : loose)++;
+  }
+  // sizes of a cache and of long prompts: answers without a walk over the rows
+  const int64_t tokens = 1 << 20, row = 48 * 128;
+  const StridedRows q = {0, 128, {row, 6 * 128, 128}, {tokens, 8, 4}}, k = {4 * 128, 128, {row, 6 * 128, 0}, {tokens, 8, 1}};
+  const StridedRows v = {64 * 1024, 128, {2 * 64 * 1024, 1024, 128}, {tokens, 64, 8}};
+  StridedRows keys = v;
+  keys.at = 0;
+  const bool far = rows_distinct(q) && !rows_touch(q, k) && rows_distinct(v) && !rows_touch(keys, v);
+  keys.at = 1024;
+  std::puts(far && rows_touch(keys, v) && met > 1000 && apart > 1000 && close > 1000 && loose > 1000 ? "ok" : "large");
+}
+"""
+
+
+def test_rows_that_overlap_are_told_from_rows_that_do_not(tmp_path):
+    """csrc/strided_rows.h against sets of small numbers, in any order and nesting of strides."""
+    if shutil.which("g++") is None:
+        pytest.skip("needs g++")
+    src, exe = tmp_path / "rows.cpp", tmp_path / "rows"
+    src.write_text(OVERLAPS)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover",
+                    "-I", os.path.join(ROOT, "yirage_b200", "csrc"), "-o", str(exe), str(src)], check=True)
+    assert subprocess.run([str(exe)], capture_output=True, text=True).stdout.strip() == "ok"
+
+
+def test_written_rows_that_share_memory_are_refused(native_lib):
+    """Strides that are wide enough one by one and still lead to the same place twice."""
+    c, lib = cache(), native_lib
+    r = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)
+    q, k = r(2, 8, 128), r(2, 2, 128)
+    for out in (r(4096).as_strided((2, 8, 128), (128, 128, 1)), r(4096).as_strided((2, 8, 128), (256, 128, 1)),
+                r(4096).as_strided((2, 2, 4, 128), (1024, 384, 128, 1))):
+        with pytest.raises(ValueError, match="must not overlap"):
+            c.decode(q.view(out.shape), out=out)
+        with pytest.raises(ValueError, match="must not overlap"):
+            c.append(k, k, q=q.view(out.shape), q_out=out)
+    for out in (r(4096).as_strided((2, 8, 128), (128, 256, 1)), r(9000).as_strided((2, 2, 4, 128), (512, 2048, 128, 1))):
+        with pytest.raises(RuntimeError, match="no CPU execution path"):      # heads in front of tokens: apart
+            c.decode(q.view(out.shape), out=out)
+
+    def append(code, text, c=None, **kw):
+        a = N.PagedAppendArgs(k=0x1000000, v=0x1000200, k_stride_token=512, k_stride_head=256, v_stride_token=512,
+                              v_stride_head=256, num_tokens=2, **kw)
+        assert lib.ypk_paged_append(C.byref(c or c_cache()), C.byref(a), None) == code
+        assert text in lib.ypk_last_error(None).decode(), lib.ypk_last_error(None)
+
+    heads = dict(num_q_heads=8, q_stride_token=1024, q_stride_group=512, q_stride_head=128, q_out_stride_token=1024,
+                 q_out_stride_group=512, q_out_stride_head=128)
+    append(N.ERR_INVALID, "rows of the cache overlap", c_cache(stride_token=128))
+    append(N.ERR_INVALID, "rows of the cache overlap", c_cache(stride_page=256))
+    append(N.ERR_INVALID, "K and V rows", c_cache(v=0x10000))
+    append(N.ERR_INVALID, "K and V rows", c_cache(v=0x10000 + 16 * 512))
+    append(N.ERR_INVALID, "rows of q_out overlap", q=0x400000, q_out=0x400000,
+           **dict(heads, q_stride_token=0, q_out_stride_token=0))
+    append(N.ERR_INVALID, "rows of q_out overlap", q=0x400000, q_out=0x500000, **dict(heads, q_out_stride_token=512))
+    append(N.ERR_INVALID, "q_out overlaps q without", q=0x400000, q_out=0x400000 + 2 * 512, **heads)
+    append(N.ERR_INVALID, "q_out overlaps k or v", q=0x400000, q_out=0x1000000 - 16, **heads)
+    append(N.ERR_INVALID, "q_out overlaps the cache", q=0x400000, q_out=0x20000 + 16, **heads)
+
+    def decode(code, text, **kw):
+        a = N.PagedDecodeArgs(**dict(dict(q=0x400000, out=0x500000, q_stride_token=1024, q_stride_group=512,
+                                          q_stride_head=128, out_stride_token=1024, out_stride_group=512,
+                                          out_stride_head=128, rows=2, num_q_heads=8, scale=0.1), **kw))
+        assert lib.ypk_paged_decode(C.byref(c_cache()), C.byref(a), None) == code
+        assert text in lib.ypk_last_error(None).decode(), lib.ypk_last_error(None)
+
+    decode(N.ERR_INVALID, "rows of out overlap", out_stride_token=512)
+    decode(N.ERR_INVALID, "out overlaps the cache", out=0x10000 + 16)
+    decode(N.ERR_INVALID, "out overlaps q", out=0x400000 + 2 * 3 * 128)

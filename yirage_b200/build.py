@@ -74,7 +74,7 @@ def build(force=False, verbose=False):
         if not os.path.exists(nvcc):
             raise RuntimeError("nvcc not found; the native library cannot be built")
         _run([nvcc] + NVCC_FLAGS + ["-o", LIB] + sources() + ["-lcudart"], verbose, "nvcc building libypk.so")
-    if force or _stale(BINDING, [BINDING_SOURCE]):
+    if force or _stale(BINDING, [BINDING_SOURCE, os.path.join(CSRC, "strided_rows.h")]):
         _run(_binding_command(), verbose, "g++ building _serving.so")
     return LIB
 

@@ -30,6 +30,12 @@ int paged_check(const char *what, const ypk_paged_cache *c, bool append) {
       (c->num_kv_heads > 1 && c->stride_head < c->head_dim))
     return op_fail(YPK_ERR_INVALID, "%s: rows of the cache overlap (strides %lld %lld %lld)", what,
                    (long long)c->stride_page, (long long)c->stride_token, (long long)c->stride_head);
+  if (!append) return YPK_OK;
+  if (!rows_distinct(cache_rows(c, c->k)))
+    return op_fail(YPK_ERR_INVALID, "%s: rows of the cache overlap (strides %lld %lld %lld)", what,
+                   (long long)c->stride_page, (long long)c->stride_token, (long long)c->stride_head);
+  if (rows_touch(cache_rows(c, c->k), cache_rows(c, c->v)))
+    return op_fail(YPK_ERR_INVALID, "%s: K and V rows of the cache overlap", what);
   return YPK_OK;
 }
 
@@ -351,11 +357,20 @@ extern "C" int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_ap
   const int group = p->q ? p->num_q_heads / cache->num_kv_heads : 1;
   if (p->q) {
     // in place or apart: a row is read by the threads that write it, and ahead of that by nobody
-    const HeadRows q = {p->q, p->q_stride_token, p->q_stride_group, p->q_stride_head};
-    const HeadRows out = {p->q_out, p->q_out_stride_token, p->q_out_stride_group, p->q_out_stride_head};
-    const bool same = q.at == out.at && q.token == out.token && q.group == out.group && q.head == out.head;
-    if (!same && heads_touch(q, out, p->num_tokens, cache->num_kv_heads, group, cache->head_dim))
+    const auto rows = [&](const void *at, int64_t token, int64_t kv, int64_t head, int heads) {
+      return head_rows(at, p->num_tokens, token, cache->num_kv_heads, kv, heads, head, cache->head_dim);
+    };
+    const StridedRows out = rows(p->q_out, p->q_out_stride_token, p->q_out_stride_group, p->q_out_stride_head, group);
+    const bool same = p->q == p->q_out && p->q_stride_token == p->q_out_stride_token &&
+                      p->q_stride_group == p->q_out_stride_group && p->q_stride_head == p->q_out_stride_head;
+    if (!same && rows_touch(rows(p->q, p->q_stride_token, p->q_stride_group, p->q_stride_head, group), out))
       return op_fail(YPK_ERR_INVALID, "paged_append: q_out overlaps q without being q");
+    if (!rows_distinct(out)) return op_fail(YPK_ERR_INVALID, "paged_append: rows of q_out overlap");
+    if (rows_touch(rows(p->k, p->k_stride_token, p->k_stride_head, 0, 1), out) ||
+        rows_touch(rows(p->v, p->v_stride_token, p->v_stride_head, 0, 1), out))
+      return op_fail(YPK_ERR_INVALID, "paged_append: q_out overlaps k or v");
+    if (rows_touch(cache_rows(cache, cache->k), out) || rows_touch(cache_rows(cache, cache->v), out))
+      return op_fail(YPK_ERR_INVALID, "paged_append: q_out overlaps the cache");
   }
   AppendArgs a;
   a.c = paged_view(cache);

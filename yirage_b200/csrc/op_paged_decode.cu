@@ -1069,10 +1069,16 @@ extern "C" int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_de
     if (s < 0 || s % 8) return op_fail(YPK_ERR_INVALID, "paged_decode: rows must start on 16-byte boundaries");
   if (!op_aligned16(p->q) || !op_aligned16(p->out) || !op_aligned16(p->workspace))
     return op_fail(YPK_ERR_INVALID, "paged_decode: an operand is not 16-byte aligned");
-  const HeadRows q = {p->q, p->q_stride_token, p->q_stride_group, p->q_stride_head};
-  const HeadRows out = {p->out, p->out_stride_token, p->out_stride_group, p->out_stride_head};
-  if (heads_touch(q, out, p->rows, cache->num_kv_heads, p->num_q_heads / cache->num_kv_heads, cache->head_dim))
+  const auto rows = [&](const void *at, int64_t token, int64_t group, int64_t head) {
+    return head_rows(at, p->rows, token, cache->num_kv_heads, group, p->num_q_heads / cache->num_kv_heads, head,
+                     cache->head_dim);
+  };
+  const StridedRows out = rows(p->out, p->out_stride_token, p->out_stride_group, p->out_stride_head);
+  if (rows_touch(rows(p->q, p->q_stride_token, p->q_stride_group, p->q_stride_head), out))
     return op_fail(YPK_ERR_INVALID, "paged_decode: out overlaps q");
+  if (!rows_distinct(out)) return op_fail(YPK_ERR_INVALID, "paged_decode: rows of out overlap");
+  if (rows_touch(cache_rows(cache, cache->k), out) || rows_touch(cache_rows(cache, cache->v), out))
+    return op_fail(YPK_ERR_INVALID, "paged_decode: out overlaps the cache");
   DeviceInfo dev;
   if (int rc = device_info(&dev)) return rc;
   DecodeArgs a;

@@ -23,6 +23,7 @@
 #include <algorithm>
 
 #include "../../include/ypk.h"
+#include "strided_rows.h"
 
 namespace {
 
@@ -162,7 +163,7 @@ Queries queries(const Cache &k, const Tensor &t, const char *name, bool written)
            name, (long long)k.dim, (long long)k.heads, (long long)k.dim, (long long)k.heads);
   q.rows = t.size(0);
   if (q.rows > 0x7fffffff || q.heads > 0x7fffffff) refuse(PyExc_ValueError, "%s is too large", name);
-  if (written && ((q.rows > 1 && st < k.dim) || (k.heads > 1 && sg < k.dim) || (group > 1 && sh < k.dim)))
+  if (written && !ypk::rows_distinct({0, k.dim, {st, sg, sh}, {q.rows, k.heads, group}}))
     refuse(PyExc_ValueError, "%s is written: its rows must not overlap", name);
   q.token = q.rows > 1 ? st : 0;
   q.group = k.heads > 1 ? sg : 0;
