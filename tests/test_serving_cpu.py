@@ -465,3 +465,12 @@ def test_written_rows_that_share_memory_are_refused(native_lib):
     decode(N.ERR_INVALID, "rows of out overlap", out_stride_token=512)
     decode(N.ERR_INVALID, "out overlaps the cache", out=0x10000 + 16)
     decode(N.ERR_INVALID, "out overlaps q", out=0x400000 + 2 * 3 * 128)
+
+
+def test_launches_are_sized_by_the_device():
+    """No SM count stands in the code of the operators: it is the current device's."""
+    csrc = os.path.join(ROOT, "yirage_b200", "csrc")
+    for name in ("op_paged_append.cu", "op_paged_decode.cu", "op_logprobs.cu"):
+        with open(os.path.join(csrc, name)) as f:
+            code = "\n".join(line.split("//")[0] for line in f)
+        assert "148" not in code and "op_device(" in code, name

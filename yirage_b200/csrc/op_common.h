@@ -9,6 +9,12 @@ namespace ypk {
 // Sets the message that ypk_last_error(NULL) returns on this thread; gives `code` back.
 int op_fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
 
+// The current device and its SM count, asked for once per device.
+struct DeviceInfo {
+  int device, sms;
+};
+int op_device(const char *what, DeviceInfo *d);
+
 inline bool op_aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Launches kernel(args) on clusters of `cluster` CTAs (0: none), set up while the kernel before it on

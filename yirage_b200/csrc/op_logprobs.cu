@@ -706,15 +706,15 @@ int cluster_size(int rows, int vocab, int sms) {
 }
 
 template <int DTYPE, bool TOP, int THREADS>
-int launch_shape(const LogprobArgs &a, int rows, int device, int sms, cudaStream_t st) {
+int launch_shape(const LogprobArgs &a, int rows, const DeviceInfo &dev, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};      // devices where clusters of sixteen have been asked for
   auto *kernel = token_logprobs_kernel<DTYPE, TOP, THREADS>;
-  if (!(ready.load(std::memory_order_relaxed) >> device & 1)) {
+  if (!(ready.load(std::memory_order_relaxed) >> dev.device & 1)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: set-up: %s", cudaGetErrorString(e));
-    ready.fetch_or(uint64_t(1) << device, std::memory_order_relaxed);
+    ready.fetch_or(uint64_t(1) << dev.device, std::memory_order_relaxed);
   }
-  const int c = cluster_size(rows, a.vocab, sms);
+  const int c = cluster_size(rows, a.vocab, dev.sms);
   return op_launch("token_logprobs", kernel, dim3(unsigned(rows) * c), THREADS, 0, c, st, a);
 }
 
@@ -723,20 +723,11 @@ int launch_shape(const LogprobArgs &a, int rows, int device, int sms, cudaStream
 // 182 against 189; 333 x 50021 19.0 against 18.4).
 template <int DTYPE>
 int launch_logprobs(const LogprobArgs &a, int rows, cudaStream_t st) {
-  static std::atomic<int> sms_of[64];
-  int device = -1;
-  cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess || device < 0 || device >= 64)
-    return op_fail(YPK_ERR_CUDA, "token_logprobs: no current device (%s)", cudaGetErrorString(e));
-  int sms = sms_of[device].load(std::memory_order_relaxed);
-  if (!sms) {
-    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "token_logprobs: SM count: %s", cudaGetErrorString(e));
-    sms_of[device].store(sms, std::memory_order_relaxed);
-  }
-  if (!a.top) return launch_shape<DTYPE, false, 256>(a, rows, device, sms, st);
-  return rows > 4 * sms ? launch_shape<DTYPE, true, 128>(a, rows, device, sms, st)
-                        : launch_shape<DTYPE, true, 256>(a, rows, device, sms, st);
+  DeviceInfo dev;
+  if (int rc = op_device("token_logprobs", &dev)) return rc;
+  if (!a.top) return launch_shape<DTYPE, false, 256>(a, rows, dev, st);
+  return rows > 4 * dev.sms ? launch_shape<DTYPE, true, 128>(a, rows, dev, st)
+                        : launch_shape<DTYPE, true, 256>(a, rows, dev, st);
 }
 
 }  // namespace

@@ -287,17 +287,19 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kern
 template <class T, bool WIDE_TABLE, int D>
 int launch_shape(AppendArgs &a, cudaStream_t st) {
   constexpr int kItems = kAppendThreads / (D / 16);
-  constexpr int kResident = 148 * kAppendCtas;
+  DeviceInfo dev;
+  if (int rc = op_device("paged_append", &dev)) return rc;
+  const int resident = dev.sms * kAppendCtas;
   const int heads = a.q_heads + 2 * a.c.kv_heads;
   const auto parts = [&](int n) { return (heads + n - 1) / n; };
-  const bool few = int64_t(a.tokens) * parts(kItems) <= kResident;
+  const bool few = int64_t(a.tokens) * parts(kItems) <= resident;
   a.heads_per_cta = std::min(heads, few ? kItems : kItems * kAhead);
   a.groups_per_token = (heads + kAhead - 1) / kAhead;
   a.rows_at_once = few ? 1 : std::max(1, kItems / a.groups_per_token);
   const int64_t units = int64_t(a.tokens) * parts(a.heads_per_cta);
   const auto over = [&](int64_t n, int64_t d) { return (n + d * a.rows_at_once - 1) / (d * a.rows_at_once); };
-  const int64_t waves = over(units, int64_t(kResident) * kMaxTurns);
-  a.rows_per_cta = std::min(int(over(units, kResident * waves)) * a.rows_at_once, kMaxRows);
+  const int64_t waves = over(units, int64_t(resident) * kMaxTurns);
+  a.rows_per_cta = std::min(int(over(units, resident * waves)) * a.rows_at_once, kMaxRows);
   const dim3 grid(unsigned((int64_t(a.tokens) + a.rows_per_cta - 1) / a.rows_per_cta), parts(a.heads_per_cta));
   if (grid.y > 65535) return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d heads", heads);
   return op_launch("paged_append",

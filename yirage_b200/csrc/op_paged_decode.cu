@@ -935,25 +935,6 @@ int n_tiles(int head_dim, int group) { return head_dim <= 128 && group > 8 ? 2 :
 
 int pass_heads(int head_dim, int group) { return std::min(group, 8 * n_tiles(head_dim, group)); }
 
-struct DeviceInfo {
-  int device, sms;
-};
-
-// SM count of the current device, asked for once per device.
-int device_info(DeviceInfo *d) {
-  static std::atomic<int> sms_of[64];
-  cudaError_t e = cudaGetDevice(&d->device);
-  if (e != cudaSuccess || d->device < 0 || d->device >= 64)
-    return op_fail(YPK_ERR_CUDA, "paged_decode: no current device (%s)", cudaGetErrorString(e));
-  d->sms = sms_of[d->device].load(std::memory_order_relaxed);
-  if (!d->sms) {
-    e = cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, d->device);
-    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "paged_decode: SM count: %s", cudaGetErrorString(e));
-    sms_of[d->device].store(d->sms, std::memory_order_relaxed);
-  }
-  return YPK_OK;
-}
-
 uint64_t workspace_bytes(int workers, int heads, int head_dim) {
   return uint64_t(workers) * (16 + 2 * uint64_t(heads) * (8 + 4 * uint64_t(head_dim)));
 }
@@ -1046,7 +1027,7 @@ extern "C" int ypk_paged_decode_workspace(const ypk_paged_cache *cache, int32_t 
   if (int rc = check_heads(cache, num_q_heads)) return rc;
   if (!bytes) return op_fail(YPK_ERR_INVALID, "paged_decode: null size");
   DeviceInfo dev;
-  if (int rc = device_info(&dev)) return rc;
+  if (int rc = op_device("paged_decode", &dev)) return rc;
   const int group = num_q_heads / cache->num_kv_heads, heads = pass_heads(cache->head_dim, group);
   const int passes = cache->num_kv_heads * ((group + heads - 1) / heads);
   // (fewer rows and a window only make clusters likelier)
@@ -1080,7 +1061,7 @@ extern "C" int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_de
   if (rows_touch(cache_rows(cache, cache->k), out) || rows_touch(cache_rows(cache, cache->v), out))
     return op_fail(YPK_ERR_INVALID, "paged_decode: out overlaps the cache");
   DeviceInfo dev;
-  if (int rc = device_info(&dev)) return rc;
+  if (int rc = op_device("paged_decode", &dev)) return rc;
   DecodeArgs a;
   a.c = paged_view(cache);
   a.q = static_cast<const char *>(p->q);

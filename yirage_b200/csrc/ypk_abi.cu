@@ -12,6 +12,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
 #include <vector>
 
@@ -122,6 +123,21 @@ int op_fail(int code, const char *fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   return fail(nullptr, code, "%s", buf);
+}
+
+int op_device(const char *what, DeviceInfo *d) {
+  static std::atomic<int> sms_of[64];
+  d->device = -1;
+  cudaError_t e = cudaGetDevice(&d->device);
+  if (e != cudaSuccess || d->device < 0 || d->device >= 64)
+    return op_fail(YPK_ERR_CUDA, "%s: no current device (%s)", what, cudaGetErrorString(e));
+  d->sms = sms_of[d->device].load(std::memory_order_relaxed);
+  if (!d->sms) {
+    e = cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, d->device);
+    if (e != cudaSuccess) return op_fail(YPK_ERR_CUDA, "%s: SM count: %s", what, cudaGetErrorString(e));
+    sms_of[d->device].store(d->sms, std::memory_order_relaxed);
+  }
+  return YPK_OK;
 }
 
 }  // namespace ypk
