@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -474,3 +475,31 @@ def test_launches_are_sized_by_the_device():
         with open(os.path.join(csrc, name)) as f:
             code = "\n".join(line.split("//")[0] for line in f)
         assert "148" not in code and "op_device(" in code, name
+
+
+def test_the_native_library_builds_without_what_the_python_binding_needs(native_lib, monkeypatch, tmp_path, capsys):
+    """A C host has nvcc alone: libypk.so is built, the binding left out with a message; a binding of
+    older sources does not stay behind.  A compiler that fails is an error all the same."""
+    from yirage_b200 import build
+    ran, binding = [], tmp_path / "_serving.so"
+    monkeypatch.setattr(build, "LIB", str(tmp_path / "libypk.so"))
+    monkeypatch.setattr(build, "BINDING", str(binding))
+    monkeypatch.setattr(build, "_run", lambda cmd, verbose, what: ran.append(what))
+    which = shutil.which
+    monkeypatch.setattr(build.shutil, "which", lambda name: None if name == "g++" else which(name))
+    binding.write_text("old")
+    os.utime(binding, (0, 0))
+    assert build.build() == build.LIB and ran == ["nvcc building libypk.so"]
+    assert "no g++" in capsys.readouterr().err and not binding.exists()
+    monkeypatch.setattr(build.shutil, "which", which)
+    for lacking in ("torch", "Python's headers"):
+        with monkeypatch.context() as m:
+            if lacking == "torch":
+                m.setitem(sys.modules, "torch", None)
+            else:
+                m.setattr(build.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+            assert build._binding_lacks() == lacking
+    if which("g++"):
+        ran.clear()
+        build.build()
+        assert ran == ["nvcc building libypk.so", "g++ building _serving.so"]

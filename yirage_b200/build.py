@@ -66,8 +66,25 @@ def _binding_command():
             "-ltorch_cuda", "-ltorch_cpu", "-lc10_cuda", "-lc10", "-Wl,-rpath,$ORIGIN"]
 
 
+def _binding_lacks():
+    """What the Python binding needs and this machine has not, or None."""
+    if shutil.which("g++") is None:
+        return "g++"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers"
+    try:
+        import torch
+    except ImportError:
+        return "torch"
+    if not os.path.isdir(os.path.join(os.path.dirname(torch.__file__), "include", "torch")):
+        return "torch's headers"
+    return None
+
+
 def build(force=False, verbose=False):
-    """Compile libypk.so and _serving.so where missing or older than their sources."""
+    """Compile libypk.so and _serving.so where missing or older than their sources.  libypk.so, all
+    that a C host needs, takes nvcc alone; where what the Python binding takes is missing, that is
+    left out with a message and serving.py raises when it is used."""
     native = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if not f.endswith(".cpp")]
     if force or _stale(LIB, native):
         nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
@@ -75,7 +92,13 @@ def build(force=False, verbose=False):
             raise RuntimeError("nvcc not found; the native library cannot be built")
         _run([nvcc] + NVCC_FLAGS + ["-o", LIB] + sources() + ["-lcudart"], verbose, "nvcc building libypk.so")
     if force or _stale(BINDING, [BINDING_SOURCE, os.path.join(CSRC, "strided_rows.h")]):
-        _run(_binding_command(), verbose, "g++ building _serving.so")
+        lacking = _binding_lacks()
+        if lacking is None:
+            _run(_binding_command(), verbose, "g++ building _serving.so")
+        else:
+            if os.path.exists(BINDING):      # of other sources: its structures may not be today's
+                os.remove(BINDING)
+            sys.stderr.write(f"_serving.so, the Python binding of the serving operators, is not built: no {lacking}\n")
     return LIB
 
 
