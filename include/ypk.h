@@ -468,6 +468,10 @@ typedef struct ypk_paged_append_args {
  * without touching are apart. */
 int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_append_args *args, void *stream);
 
+/* Takes the error bits: *taken = *cache->status and *cache->status = 0 in one step, so that a bit that
+ * a call on another stream sets meanwhile is in this or in the next take.  Both on the device. */
+int ypk_paged_status(const ypk_paged_cache *cache, int32_t *taken, void *stream);
+
 /* Operands of ypk_paged_decode. */
 typedef struct ypk_paged_decode_args {
   const void *q;                /* [rows][group..][head_dim], grouped as in ypk_paged_append */

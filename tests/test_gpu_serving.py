@@ -1233,3 +1233,29 @@ def test_queries_and_outputs_side_by_side_in_one_buffer():
     assert torch.equal(same.decode(q), yr.PagedKVCache(b.k, b.k.clone(), b.meta).decode(q))
     with pytest.raises(N.YpkError, match="K and V rows"):
         same.append(k, v)
+
+
+def test_check_misses_nothing_of_another_stream():
+    """A bit that a call on another stream sets while check() reads and clears those of this one is in that
+    check or in the next one."""
+    b = Batch([60, 60], page=16, seed=15)
+    q = rnd(gen(16), 2, 8, 128)
+    b.meta["paged_kv_last_page_len_buffer"][0] = 17                   # request 0: a table out of order
+    b.meta["paged_kv_indices_buffer"][int(b.meta["paged_kv_indptr_buffer"][1])] = -1     # 1: a bad page
+    torch.cuda.synchronize()
+    side, slow = torch.cuda.Stream(), torch.randn(1024, 1024, device="cuda")
+    for turn in range(200):
+        with torch.cuda.stream(side):
+            for _ in range(turn % 5 + 1):
+                slow @ slow
+            b.cache.decode(q)
+            done = side.record_event()
+        found, last = 0, False
+        while not last:
+            last = done.query()
+            b.cache.decode(q[:1])
+            with pytest.raises(N.YpkError, match="out of order") as e:
+                b.cache.check()
+            found += "outside the pool" in str(e.value)
+        assert found == 1, turn
+    b.cache.check()

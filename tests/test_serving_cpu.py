@@ -503,3 +503,10 @@ def test_the_native_library_builds_without_what_the_python_binding_needs(native_
         ran.clear()
         build.build()
         assert ran == ["nvcc building libypk.so", "g++ building _serving.so"]
+
+
+def test_taking_the_status_refuses_null(native_lib):
+    for c, taken in ((None, 0x1000), (c_cache(), 0x1000), (c_cache(status=0x1000), None)):
+        assert native_lib.ypk_paged_status(c and C.byref(c), taken, None) == N.ERR_INVALID
+        assert "paged_status: null" in native_lib.ypk_last_error(None).decode()
+    assert cache().check() is None        # on the CPU nothing has run

@@ -163,6 +163,7 @@ SYMBOLS = {
     "ypk_argmax_noalloc": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_int64, C.c_void_p,
                                      C.c_void_p]),
     "ypk_paged_append": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedAppendArgs), C.c_void_p]),
+    "ypk_paged_status": (C.c_int, [C.POINTER(PagedCache), C.c_void_p, C.c_void_p]),
     "ypk_paged_decode": (C.c_int, [C.POINTER(PagedCache), C.POINTER(PagedDecodeArgs), C.c_void_p]),
     "ypk_paged_decode_workspace": (C.c_int, [C.POINTER(PagedCache), C.c_int32,
                                              C.POINTER(C.c_uint64)]),

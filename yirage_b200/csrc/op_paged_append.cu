@@ -315,6 +315,14 @@ int launch_append(int head_dim, AppendArgs &a, cudaStream_t st) {
   return launch_shape<T, WIDE_TABLE, 256>(a, st);
 }
 
+struct StatusArgs {
+  int *status, *taken;
+};
+__global__ void paged_status_kernel(const __grid_constant__ StatusArgs a) {
+  op_wait_for_previous();
+  *a.taken = atomicExch(a.status, 0);
+}
+
 bool strides_ok(std::initializer_list<int64_t> s) {
   for (int64_t v : s)
     if (v < 0 || v % 8) return false;
@@ -325,6 +333,12 @@ bool strides_ok(std::initializer_list<int64_t> s) {
 }  // namespace ypk
 
 using namespace ypk;
+
+extern "C" int ypk_paged_status(const ypk_paged_cache *cache, int32_t *taken, void *stream) {
+  if (!cache || !cache->status || !taken) return op_fail(YPK_ERR_INVALID, "paged_status: null cache, status or result");
+  return op_launch("paged_status", paged_status_kernel, dim3(1), 1, 0, 0, static_cast<cudaStream_t>(stream),
+                   StatusArgs{cache->status, taken});
+}
 
 extern "C" int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_append_args *p, void *stream) {
   if (int rc = paged_check("paged_append", cache, true)) return rc;

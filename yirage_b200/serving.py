@@ -128,11 +128,17 @@ class PagedKVCache:
 
     def check(self):
         """Wait for the work enqueued so far on the current stream and raise if a call found a
-        broken table entry since the last check."""
-        bits = int(self.status.item())
+        broken table entry since the last check.  The bits are taken in one step: what a call on
+        another stream finds meanwhile is left for the next check."""
+        if self._index < 0:
+            return
+        with torch.cuda.device(self._index):
+            taken = torch.empty_like(self.status)
+            N.check(None, N.load().ypk_paged_status(C.byref(self._c), C.c_void_p(taken.data_ptr()),
+                                                    C.c_void_p(torch.cuda.current_stream().cuda_stream)))
+        bits = int(taken.item())
         if not bits:
             return
-        self.status.zero_()
         what = [text for bit, text in ((N.PAGED_BAD_TABLE, "page offsets or a last page length out of order"),
                                        (N.PAGED_BAD_PAGE, "a page number outside the pool"),
                                        (N.PAGED_BAD_POSITION, "a position outside the rotary tables"),
