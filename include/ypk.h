@@ -434,8 +434,8 @@ typedef struct ypk_paged_cache {
   int32_t num_requests, num_indices;
 } ypk_paged_cache;
 
-/* Operands of ypk_paged_append.  Strides in elements, each a multiple of 8; pointers 16-byte
- * aligned; the head dimension is contiguous everywhere.  Query head h is head h % group of group
+/* Operands of ypk_paged_append.  Strides in elements, each a multiple of 8 (of 4 for tables in
+ * fp32); pointers 16-byte aligned; the head dimension is contiguous everywhere.  Query head h is head h % group of group
  * h / group, group = num_q_heads / num_kv_heads, so that the rows of a fused projection
  * ([q heads of the group | k | v] per K/V head) are taken as they lie. */
 typedef struct ypk_paged_append_args {

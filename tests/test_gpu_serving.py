@@ -1259,3 +1259,20 @@ def test_check_misses_nothing_of_another_stream():
             found += "outside the pool" in str(e.value)
         assert found == 1, turn
     b.cache.check()
+
+
+@pytest.mark.parametrize("dtype,table,step", [(BF16, F32, 4), (F16, F32, 12), (BF16, BF16, 8), (F16, F16, 24)])
+def test_append_table_rows_on_every_16_byte_boundary(dtype, table, step):
+    """Tables as a view into wider rows: any row that starts on a 16-byte boundary."""
+    b, c = (Batch([30, 7], [10, 7], dtype=dtype, seed=6) for _ in range(2))
+    g = gen(7)
+    k, v, q = (rnd(g, 17, h, 128, dtype=dtype) for h in (2, 2, 8))
+    cos, sin = tables(64, 128, table)
+    wide = torch.full((64, 256 + step), float("nan"), dtype=table, device="cuda")
+    wide[:, :128], wide[:, 128:256] = cos, sin
+    got = c.cache.append(k, v, q=q, cos=wide[:, :128], sin=wide[:, 128:256])
+    assert torch.equal(got, b.cache.append(k, v, q=q, cos=cos, sin=sin))
+    assert torch.equal(c.k.view(torch.int16), b.k.view(torch.int16))
+    odd = torch.zeros(64, 256 + step // 2, dtype=table, device="cuda")
+    with pytest.raises(N.YpkError, match="row stride"):
+        c.cache.append(k, v, q=q, cos=odd[:, :128], sin=odd[:, 128:256])

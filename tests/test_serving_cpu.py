@@ -510,3 +510,14 @@ def test_taking_the_status_refuses_null(native_lib):
         assert native_lib.ypk_paged_status(c and C.byref(c), taken, None) == N.ERR_INVALID
         assert "paged_status: null" in native_lib.ypk_last_error(None).decode()
     assert cache().check() is None        # on the CPU nothing has run
+
+
+def test_table_rows_in_32_bits_start_on_16_byte_boundaries(native_lib):
+    """A row stride of 4 x 4 bytes is one; what is behind the check refuses this call (an unaligned k)."""
+    for dtype, stride, text in ((N.F32, 132, "not 16-byte aligned"), (N.F32, 130, "row stride 130"),
+                                (N.BF16, 132, "row stride 132"), (N.BF16, 136, "not 16-byte aligned")):
+        a = N.PagedAppendArgs(k=0x10002, v=0x10000, k_stride_token=256, k_stride_head=128, v_stride_token=256,
+                              v_stride_head=128, num_tokens=2, cos=0x10000, sin=0x10000, table_dtype=dtype,
+                              max_positions=64, table_stride=stride, rot_dim=128)
+        assert native_lib.ypk_paged_append(C.byref(c_cache()), C.byref(a), None) == N.ERR_INVALID
+        assert text in native_lib.ypk_last_error(None).decode()

@@ -360,7 +360,7 @@ extern "C" int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_ap
                      p->rot_dim, cache->head_dim);
     if (!wide && p->table_dtype != cache->dtype)
       return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: table type %d (the cache's or fp32)", p->table_dtype);
-    if (p->max_positions < 1 || p->table_stride < p->rot_dim || p->table_stride % 8)
+    if (p->max_positions < 1 || p->table_stride < p->rot_dim || p->table_stride % (wide ? 4 : 8))
       return op_fail(YPK_ERR_INVALID, "paged_append: tables of %d positions, row stride %lld",
                      p->max_positions, (long long)p->table_stride);
   }
