@@ -521,3 +521,14 @@ def test_table_rows_in_32_bits_start_on_16_byte_boundaries(native_lib):
                               max_positions=64, table_stride=stride, rot_dim=128)
         assert native_lib.ypk_paged_append(C.byref(c_cache()), C.byref(a), None) == N.ERR_INVALID
         assert text in native_lib.ypk_last_error(None).decode()
+
+
+def test_log_probabilities_of_no_rows_are_checked_like_any(native_lib):
+    """A call without rows does nothing, with arguments that a call with rows would take."""
+    call = lambda **kw: native_lib.ypk_token_logprobs(*dict(dict(
+        logits=None, dtype=N.BF16, rows=0, vocab=100, ld=104, tokens=None, top=2, lp=None, ent=None, tl=None, tt=None,
+        stream=None), **kw).values())
+    assert call() == N.YPK_OK
+    for kw, code in ((dict(top=33), N.ERR_UNSUPPORTED), (dict(top=-1), N.ERR_UNSUPPORTED), (dict(top=5, vocab=4), N.ERR_UNSUPPORTED),
+                     (dict(dtype=N.I32), N.ERR_UNSUPPORTED), (dict(ld=99), N.ERR_INVALID), (dict(vocab=0), N.ERR_INVALID)):
+        assert call(**kw) == code, kw

@@ -738,9 +738,6 @@ using namespace ypk;
 extern "C" int ypk_token_logprobs(const void *logits, int32_t dtype, int32_t rows, int32_t vocab, int64_t ld,
                                   const int64_t *tokens, int32_t top_k, float *logprob, float *entropy,
                                   float *top_logprob, int64_t *top_token, void *stream) {
-  if (rows == 0) return YPK_OK;
-  if (!logits || !tokens || !logprob || !entropy)
-    return op_fail(YPK_ERR_INVALID, "token_logprobs: null logits, tokens or output");
   if (dtype != YPK_BF16 && dtype != YPK_F16 && dtype != YPK_F32)
     return op_fail(YPK_ERR_UNSUPPORTED, "token_logprobs: type %d (bf16, fp16 or fp32)", dtype);
   if (rows < 0 || vocab < 1 || ld < vocab)
@@ -748,6 +745,9 @@ extern "C" int ypk_token_logprobs(const void *logits, int32_t dtype, int32_t row
                    (long long)ld);
   if (top_k < 0 || top_k > kMaxTop || top_k > vocab)
     return op_fail(YPK_ERR_UNSUPPORTED, "token_logprobs: top_k %d (0..%d, at most the vocabulary)", top_k, kMaxTop);
+  if (rows == 0) return YPK_OK;      // (nothing to read or write: pointers may be null)
+  if (!logits || !tokens || !logprob || !entropy)
+    return op_fail(YPK_ERR_INVALID, "token_logprobs: null logits, tokens or output");
   if (top_k > 0 && (!top_logprob || !top_token))
     return op_fail(YPK_ERR_INVALID, "token_logprobs: null output of the top alternatives");
   if (reinterpret_cast<uintptr_t>(logits) % (dtype == YPK_F32 ? 4 : 2))

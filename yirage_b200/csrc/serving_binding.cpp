@@ -355,7 +355,7 @@ PyObject *logprobs(const void *ptr, int dtype, int64_t rows, int64_t vocab, int6
   need_cuda(device);
   const c10::cuda::CUDAGuard guard(device);
   // One allocation for the four results (a call on a few rows 4.8 us, with four 6.1).
-  const int64_t kept = rows ? std::min<int64_t>(top, 32) : top;      // (more are refused below)
+  const int64_t kept = std::min<int64_t>(top, 32);      // (more are refused below)
   const Tensor all = at::detail::empty_cuda({rows * (8 + 12 * kept)}, at::kByte, device, std::nullopt);
   int64_t at = 0;
   const auto take = [&](at::ScalarType type, at::IntArrayRef sizes) {
