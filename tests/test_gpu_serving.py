@@ -1276,3 +1276,32 @@ def test_append_table_rows_on_every_16_byte_boundary(dtype, table, step):
     odd = torch.zeros(64, 256 + step // 2, dtype=table, device="cuda")
     with pytest.raises(N.YpkError, match="row stride"):
         c.cache.append(k, v, q=q, cos=odd[:, :128], sin=odd[:, 128:256])
+
+
+def test_append_and_decode_steps_to_a_rounding():
+    """The steps of test_append_and_decode_together with the bounds of append and of decode by
+    themselves: the attention is that of the query which append returned, over what the cache holds."""
+    steps = 20
+    cos, sin = tables(256, 128, BF16)
+    b, ks, vs, qs = make_steps(20, steps=steps)
+    turned = []
+    plain = b.cache.append
+
+    def append(*args, **kw):
+        turned.append(plain(*args, **kw).clone())
+        return turned[-1]
+
+    b.cache.append = append
+    start = list(b.lengths)
+    outs = decode_loop(b, cos, sin, ks, vs, qs, steps)
+    for r in range(3):
+        at = b.where(r, torch.arange(b.lengths[r], device="cuda"))
+        k, v = b.k[at], b.v[at]
+        for i in range(steps):
+            n = start[r] + i + 1
+            for got, x in ((k[n - 1], ks[i][r]), (turned[i][r], qs[i][r])):
+                y, size = rotated64(x[None], None, 0, cos[n - 1:n], sin[n - 1:n])
+                bound = half_step(BF16) * (1 + 2 ** -6) * y.abs() + 2 * 3 * 2 ** -24 * size
+                assert ((got.to(F64) - y[0]).abs() <= bound[0]).all(), (r, i)
+            assert torch.equal(v[n - 1], vs[i][r])
+            check_attention(outs[i][r], None, turned[i][r], k[:n], v[:n], 128 ** -0.5, BF16)
