@@ -465,7 +465,7 @@ typedef struct ypk_paged_append_args {
  * were, and so do those of dropped tokens.  Two rows of a call must not go to the same place (two
  * requests that share a last page).  Refused: caches whose rows lie on one another, K on V among
  * them, and q_out on q (without being q), k, v or the cache; rows that alternate in one buffer
- * without touching are apart. */
+ * without touching are apart.  At most 65535 heads in all (q, k and v). */
 int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_append_args *args, void *stream);
 
 /* Takes the error bits: *taken = *cache->status and *cache->status = 0 in one step, so that a bit that
@@ -503,7 +503,7 @@ int ypk_paged_decode_workspace(const ypk_paged_cache *cache, int32_t num_q_heads
  * logprob[r] = log p(tokens[r]) (-infinity for a token outside [0, vocab)), entropy[r] =
  * -sum p log p in nats, and the top_k (0..32) most probable tokens in falling order, the lower
  * column first on ties: top_logprob, top_token [rows][top_k].  logits: dtype YPK_BF16, YPK_F16
- * or YPK_F32, row stride ld elements, aligned to its element; columns from vocab to ld (the
+ * or YPK_F32, at most 2^30 columns, row stride ld elements, aligned to its element; columns from vocab to ld (the
  * padding of an lm_head) are not looked at.  Columns of -infinity are ruled out; in a row that
  * has no others every log probability is -infinity and the entropy 0.  A row with a NaN or
  * +infinity gives NaN (its top tokens: NaN counts as lowest). */

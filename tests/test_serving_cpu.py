@@ -532,3 +532,17 @@ def test_log_probabilities_of_no_rows_are_checked_like_any(native_lib):
     for kw, code in ((dict(top=33), N.ERR_UNSUPPORTED), (dict(top=-1), N.ERR_UNSUPPORTED), (dict(top=5, vocab=4), N.ERR_UNSUPPORTED),
                      (dict(dtype=N.I32), N.ERR_UNSUPPORTED), (dict(ld=99), N.ERR_INVALID), (dict(vocab=0), N.ERR_INVALID)):
         assert call(**kw) == code, kw
+
+
+def test_sizes_past_32_bit_counting_are_refused(native_lib):
+    """A loop over columns steps past the last one by the threads of a block, and heads are summed: both
+    stay below 2^31.  (What would be behind the checks refuses these calls: null pointers.)"""
+    for vocab, code, text in ((2 ** 31 - 1, N.ERR_UNSUPPORTED, "vocabulary 2147483647"), (2 ** 30 + 1, N.ERR_UNSUPPORTED, "at most"),
+                              (2 ** 30, N.ERR_INVALID, "null")):
+        assert native_lib.ypk_token_logprobs(None, N.BF16, 1, vocab, vocab, None, 0, None, None, None, None, None) == code
+        assert text in native_lib.ypk_last_error(None).decode()
+    for heads, text in ((2 ** 31 - 2, "query and 2 K/V heads"), (65532, "query and"), (65530, "not 16-byte aligned")):
+        a = N.PagedAppendArgs(k=0x10002, v=0x10000, k_stride_token=256, k_stride_head=128, v_stride_token=256,
+                              v_stride_head=128, num_tokens=2, q=0x400000, q_out=0x400000, num_q_heads=heads)
+        assert native_lib.ypk_paged_append(C.byref(c_cache()), C.byref(a), None) != N.YPK_OK
+        assert text in native_lib.ypk_last_error(None).decode()

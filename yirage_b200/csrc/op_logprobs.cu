@@ -43,6 +43,7 @@ namespace ypk {
 namespace {
 
 constexpr int kMaxTop = 32;
+constexpr int kMaxVocab = 1 << 30;  // columns are counted in 32 bits, a stride of threads past the last one
 constexpr int kGroups = 64;        // of threads: what the bound of a top list is taken from
 constexpr int kMaxGroups = 128;    // over a cluster
 constexpr int kCandidates = 1024;
@@ -743,6 +744,8 @@ extern "C" int ypk_token_logprobs(const void *logits, int32_t dtype, int32_t row
   if (rows < 0 || vocab < 1 || ld < vocab)
     return op_fail(YPK_ERR_INVALID, "token_logprobs: %d rows, vocabulary %d, row stride %lld", rows, vocab,
                    (long long)ld);
+  if (vocab > kMaxVocab)
+    return op_fail(YPK_ERR_UNSUPPORTED, "token_logprobs: vocabulary %d (at most %d)", vocab, kMaxVocab);
   if (top_k < 0 || top_k > kMaxTop || top_k > vocab)
     return op_fail(YPK_ERR_UNSUPPORTED, "token_logprobs: top_k %d (0..%d, at most the vocabulary)", top_k, kMaxTop);
   if (rows == 0) return YPK_OK;      // (nothing to read or write: pointers may be null)

@@ -301,7 +301,6 @@ int launch_shape(AppendArgs &a, cudaStream_t st) {
   const int64_t waves = over(units, int64_t(resident) * kMaxTurns);
   a.rows_per_cta = std::min(int(over(units, resident * waves)) * a.rows_at_once, kMaxRows);
   const dim3 grid(unsigned((int64_t(a.tokens) + a.rows_per_cta - 1) / a.rows_per_cta), parts(a.heads_per_cta));
-  if (grid.y > 65535) return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d heads", heads);
   return op_launch("paged_append",
                    a.rows_at_once > 1 ? paged_append_kernel<T, WIDE_TABLE, D, true>
                                       : paged_append_kernel<T, WIDE_TABLE, D, false>,
@@ -350,6 +349,9 @@ extern "C" int ypk_paged_append(const ypk_paged_cache *cache, const ypk_paged_ap
     return op_fail(YPK_ERR_INVALID, "paged_append: q and q_out come together");
   if (p->q && (p->num_q_heads < 1 || p->num_q_heads % cache->num_kv_heads))
     return op_fail(YPK_ERR_INVALID, "paged_append: %d query heads over %d K/V heads", p->num_q_heads,
+                   cache->num_kv_heads);
+  if (int64_t(p->q ? p->num_q_heads : 0) + 2 * int64_t(cache->num_kv_heads) > 65535)      // (sums of them are 32-bit)
+    return op_fail(YPK_ERR_UNSUPPORTED, "paged_append: %d query and %d K/V heads", p->q ? p->num_q_heads : 0,
                    cache->num_kv_heads);
   if ((p->cos == nullptr) != (p->sin == nullptr))
     return op_fail(YPK_ERR_INVALID, "paged_append: cos and sin come together");
