@@ -23,11 +23,12 @@
 // A row is split over a cluster of CTAs when there are few rows; bounds, sums and candidates
 // travel through distributed shared memory, so there is no workspace and no second launch.
 //
-// Measured, bf16 unless said: 4096 x 128256 without alternatives 161 us = 6.5 TB/s (the copy
-// rate) while the SM clock is up, 185 to 193 us once the card's power cap has lowered it to 1.6
-// GHz (special-function unit 73 % busy, issue slots 59 %); with 20 alternatives 187.  333 x 50021
-// fp32, 8 alternatives 18 us: 12 to stream at 2.25 CTAs per SM, then 1.6 for the bound, 1.4 for the
-// candidates.  64 x 151936, 20 alternatives 11.5 us; 1 x 128256, 5 alternatives 6.7 us, latency.
+// Measured, called back to back, bf16 unless said: 4096 x 128256 without alternatives 182 to 194 us
+// = 5.4 to 5.8 TB/s, with the SM clock lowered to 1.6 GHz by the card's power cap (special-function
+// unit 73 % busy, issue slots 59 %; 161 us, the copy rate, while the clock is up); with 20
+// alternatives 187.  333 x 50021 fp32, 8 alternatives 18.7 us: 12 to stream at 2.25 CTAs per SM, as
+// a row is one CTA from 223 rows on, then 1.6 for the bound, 1.4 for the candidates.  64 x 151936, 20
+// alternatives 12.1 us; 1 x 128256, 5 alternatives 6.35 us, latency.
 // Exponentials as polynomials for a quarter of the pairs: 204 against 190 us at the cap.
 #include <cooperative_groups.h>
 #include <math.h>

@@ -143,10 +143,12 @@ __device__ __forceinline__ Place find_place(const AppendArgs &a, int row) {
 // the places are looked up.
 //
 // Bytes bound it: rows in and out once, 2 (Hq + 2 Hkv) D elements a token.  At 128 registers four
-// CTAs of 128 threads are resident, each thread with 96 bytes in flight and 96 in work.  Measured
-// (32 + 2 x 8 heads of 128, bf16): 32768 tokens 132 us = 6.1 TB/s, 93 % of the copy rate; 4498
-// tokens of 32 + 2 x 4 heads with norms 21.5 us = 4.3 TB/s, one wave whose first lookups (2 us)
-// and last stores nothing covers; one token 3.4 us, launch and five dependent loads.  Two heads a
+// CTAs of 128 threads are resident, each thread with 96 bytes in flight and 96 in work; that spills
+// 40 bytes a thread, 84 where a CTA has several tokens at once.  Measured
+// (32 + 2 x 8 heads of 128, bf16): 32768 tokens called back to back 138 us = 5.8 TB/s, 89 % of the
+// copy rate (132 us in a graph); 4498 tokens of 32 + 2 x 4 heads with norms 21.6 us = 4.3 TB/s, in
+// one wave, so that nothing covers its first lookups (2 us) and last stores; one token 3.4 us in a
+// graph, launch and five dependent loads.  Two heads a
 // thread 165 us on 32768 tokens, 256 threads a CTA 171, three CTAs per SM 152.
 template <class T, bool WIDE_TABLE, int D, bool TOGETHER>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas) paged_append_kernel(const __grid_constant__ AppendArgs a) {

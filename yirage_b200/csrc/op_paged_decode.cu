@@ -25,8 +25,8 @@
 // across that boundary.  Where the (request, head)s are many and short, each warp has a range of
 // its own instead (kManyShort) and only what crosses warps is merged, once, at the end.
 //
-// Measured, K/V heads of 128, bf16: 64 x 4096 tokens, 32 query / 8 K/V heads 164 us = 6.53 TB/s
-// (99 % of the copy rate); 8 x 4096 29 us = 4.6 TB/s, of which about 8 us are not streaming: launch
+// Measured, K/V heads of 128, bf16: 64 x 4096 tokens, 32 query / 8 K/V heads 174 to 177 us = 6.1 TB/s
+// (93 % of the copy rate; 164 while the SM clock is up); 8 x 4096 30 us = 4.5 TB/s, of which about 8 us are not streaming: launch
 // 1, lengths and range 1.5, page numbers 0.6, first rows 1.5, uneven end 2, merge and join 3;
 // 1 x 513 6.3 us, latency throughout.  What did not help: warps on different K/V heads
 // (64 x 4096 with 64 query heads 184 against 170 us), two CTAs of four warps per SM (8 x 4096 32.6
