@@ -6,11 +6,11 @@
 
 namespace ypk {
 
-// First thing in every kernel of op_launch (op_common.h): until the kernel before it on the stream
-// has ended and its writes are there.  What the kernel before may have written (inputs, page
-// tables, weights: all of it) is read behind this with ordinary loads only: a load that says its
-// data is never written (ld.global.nc, __ldg) may be moved above it, and says something untrue, as
-// this kernel is already there while the one before still writes.
+// In every kernel of op_launch (op_common.h), before it touches memory: until the kernel before it
+// on the stream has ended and its writes are there.  What the kernel before may have written
+// (inputs, page tables, weights: all of it) is read behind this with ordinary loads only: a load that
+// says its data is never written (ld.global.nc, __ldg) may be moved above it, and says something
+// untrue, as this kernel is already there while the one before still writes.
 __device__ __forceinline__ void op_wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // 16 bytes that are read once (to leave the caches first).
