@@ -493,7 +493,7 @@ typedef struct ypk_paged_decode_args {
  * out = sum_p softmax_p(scale q.k_p) v_p, lse = ln sum_p exp(scale q.k_p).  A request without
  * positions gives zeros and -infinity.  An infinity in V of a seen position is one in that
  * dimension of out, however small the position's weight (of both signs, or beside a NaN: a
- * NaN). */
+ * NaN).  A score of -infinity weighs nothing; one of +infinity or a NaN makes its head NaN. */
 int ypk_paged_decode(const ypk_paged_cache *cache, const ypk_paged_decode_args *args, void *stream);
 /* Workspace of such a call on the current device for any number of rows and any lengths; may
  * be 0. */

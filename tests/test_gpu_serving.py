@@ -1305,3 +1305,25 @@ def test_append_and_decode_steps_to_a_rounding():
                 assert ((got.to(F64) - y[0]).abs() <= bound[0]).all(), (r, i)
             assert torch.equal(v[n - 1], vs[i][r])
             check_attention(outs[i][r], None, turned[i][r], k[:n], v[:n], 128 ** -0.5, BF16)
+
+
+@pytest.mark.parametrize("lengths", [[200, 30], [9000, 40], [(29 * i) % 131 for i in range(165)] + [3000]])
+def test_decode_infinities_in_k(lengths):
+    """A score of -infinity weighs nothing, all of a head's give zeros; one of +infinity gives NaN."""
+    b = Batch(lengths, heads=2, page=16, seed=98)
+    q = rnd(gen(99), len(lengths), 8, 128)
+    q[:, 0::2, 5], q[:, 1::2, 5] = -1.0, 1.0
+    r, n = len(lengths) - 1, lengths[-1]
+    one = b.where(r, torch.tensor([n // 2], device="cuda"))
+    b.k[one[0], one[1], 0, 5] = float("inf")
+    out, lse = b.cache.decode(q, return_lse=True)
+    assert torch.isnan(out[r, 1:4:2]).all() and torch.isnan(lse[r, 1:4:2]).all()
+    rest = torch.cat((torch.arange(n // 2, device="cuda"), torch.arange(n // 2 + 1, n, device="cuda")))
+    at = b.where(r, rest)
+    check_attention(out[r, 0:4:2], lse[r, 0:4:2], q[r, 0:4:2], b.k[at][:, :1], b.v[at][:, :1], 128 ** -0.5, BF16)
+    at = b.where(r, torch.arange(n, device="cuda"))
+    check_attention(out[r, 4:], lse[r, 4:], q[r, 4:], b.k[at][:, 1:], b.v[at][:, 1:], 128 ** -0.5, BF16)
+    b.k[at[0], at[1], 0, 5] = float("inf")
+    out, lse = b.cache.decode(q, return_lse=True)
+    assert (out[r, 0:4:2] == 0).all() and (lse[r, 0:4:2] == float("-inf")).all() and torch.isnan(out[r, 1:4:2]).all()
+    check_attention(out[r, 4:], lse[r, 4:], q[r, 4:], b.k[at][:, 1:], b.v[at][:, 1:], 128 ** -0.5, BF16)
