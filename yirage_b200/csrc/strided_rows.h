@@ -50,15 +50,19 @@ inline bool rows_distinct(const StridedRows &r) {
   int n = 0;
   for (int k = 0; k < 3; ++k)
     if (r.count[k] > 1) dims[n++] = {r.stride[k], -(r.count[k] - 1), r.count[k] - 1};
+  // nested dimensions, each step over all that the narrower ones reach; most often as they stand
+  const auto nested = [&] {
+    int64_t extent = r.width;
+    for (int i = n - 1; i >= 0; --i) {
+      if (dims[i].stride < extent) return false;
+      extent += dims[i].hi * dims[i].stride;
+    }
+    return true;
+  };
+  if (nested()) return true;
   widest_first(dims, n);
-  int64_t extent = r.width;
-  bool nested = true;
-  for (int i = n - 1; i >= 0; --i) {
-    nested &= dims[i].stride >= extent;
-    extent += dims[i].hi * dims[i].stride;
-  }
   int budget = 1 << 16;
-  return nested || !some_step_meets(dims, n, 0, r.width, false, budget);
+  return nested() || !some_step_meets(dims, n, 0, r.width, false, budget);
 }
 
 // Some row of a shares a unit with one of b (the same width); also where that is too tangled to tell.
